@@ -57,6 +57,16 @@ class FfaPeerArgs(C.Structure):
                 ("peer_gathered", C.POINTER(C.c_void_p)), ("peer_flags", C.POINTER(C.c_void_p))]
 
 
+class FfaPageTable(C.Structure):
+    _fields_ = [("n_pages", C.c_int32), ("max_seqs", C.c_int32), ("cols", C.c_int32), ("bt_stride", C.c_int32),
+                ("block_table", C.c_void_p), ("seq_lens", C.c_void_p), ("refcount", C.c_void_p), ("status", C.c_void_p),
+                ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t)]
+
+
+class FfaPagePools(C.Structure):
+    _fields_ = [("n_pools", C.c_int32), ("max_token_bytes", C.c_int32), ("bases", C.c_void_p), ("token_bytes", C.c_void_p)]
+
+
 class FfaKprojArgs(C.Structure):
     _fields_ = [
         ("variant", C.c_int32),
@@ -119,6 +129,17 @@ def lib() -> C.CDLL:
         getattr(L, name).restype = C.c_int
     L.ffa_quantize_append.argtypes = [i32, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp]
     L.ffa_quantize_append.restype = C.c_int
+    L.ffa_cache_append_ragged.argtypes = [vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp, i32, i32, vp, vp, vp]
+    L.ffa_cache_append_ragged.restype = C.c_int
+    table, pools = C.POINTER(FfaPageTable), C.POINTER(FfaPagePools)
+    L.ffa_pages_scratch_bytes.argtypes = [i32, i32]
+    L.ffa_pages_scratch_bytes.restype = C.c_size_t
+    L.ffa_pages_truncate.argtypes = [table, vp, vp, i32, vp]
+    L.ffa_pages_fork.argtypes = [table, vp, vp, i32, vp]
+    L.ffa_pages_extend.argtypes = [table, pools, vp, vp, i32, vp]
+    L.ffa_pages_compact.argtypes = [table, pools, vp, vp, vp]
+    for name in ("ffa_pages_truncate", "ffa_pages_fork", "ffa_pages_extend", "ffa_pages_compact"):
+        getattr(L, name).restype = C.c_int
     L.ffa_kproj_rope.argtypes = [C.POINTER(FfaKprojArgs), C.c_void_p]
     L.ffa_kproj_rope.restype = C.c_int
     L.ffa_kproj_workspace_bytes.argtypes = [i32, i32, i32, i32]
@@ -158,3 +179,12 @@ def ptr(t) -> int | None:
 
 def current_stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def enqueue(device: torch.device, fn, what: str, *args) -> None:
+    """Call ``fn(*args, stream)`` on ``device`` and its current stream, whichever device is the current one."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)

@@ -368,6 +368,50 @@ __global__ void __launch_bounds__(256) nvfp4_kernel(const void* __restrict__ k, 
   }
 }
 
+// K and V of new tokens to each sequence's own position.  A thread takes eight channels of one token: quantises K,
+// copies V.  Four tokens' loads are in flight per thread.  Tokens past counts[b], and positions without a page, are
+// left out: nothing is written for them.
+template <int DT, int F8>
+__global__ void __launch_bounds__(256) append_ragged_kernel(const void* __restrict__ k, const uint4* __restrict__ v,
+                                                            int64_t n_vec, int groups_per_row, int T,
+                                                            const int32_t* __restrict__ positions,
+                                                            const int32_t* __restrict__ counts,
+                                                            const int32_t* __restrict__ table, int stride, int cols,
+                                                            int n_pages, uint8_t* __restrict__ base,
+                                                            uint8_t* __restrict__ res, uint4* __restrict__ v_pool) {
+  constexpr int U = 4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i0 < n_vec; i0 += U * step) {
+    int64_t out[U];
+    float x[U][8];
+    uint4 vv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = i0 + u * step;
+      out[u] = -1;
+      if (i >= n_vec) continue;
+      const int64_t row = i / groups_per_row;
+      const int g = static_cast<int>(i - row * groups_per_row);
+      const int b = static_cast<int>(row / T), tt = static_cast<int>(row - static_cast<int64_t>(b) * T);
+      if (counts && tt >= counts[b]) continue;
+      const int64_t pos = static_cast<int64_t>(positions[b]) + tt;
+      if (pos < 0 || pos >= static_cast<int64_t>(cols) * kPage) continue;
+      const int page = table[static_cast<int64_t>(b) * stride + pos / kPage];
+      if (page < 0 || page >= n_pages) continue;
+      out[u] = (static_cast<int64_t>(page) * kPage + pos % kPage) * groups_per_row + g;
+      load8<DT>(k, i * 8, x[u]);
+      vv[u] = v[i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (out[u] < 0) continue;
+      const float none[8] = {};
+      encode8<kEncFp8, DT, F8>(x[u], none, none, 0.f, base, res, out[u], true);
+      v_pool[out[u]] = vv[u];
+    }
+  }
+}
+
 int check_common(const void* k, int dt, int B, int T, int HKV, int fp8) {
   if (!k) return FFA_E_NULL;
   if (B <= 0 || T <= 0 || HKV <= 0) return FFA_E_SHAPE;
@@ -586,6 +630,30 @@ extern "C" int ffa_cache_append(int32_t variant, const void* k, const void* v, i
     return last_launch("ffa_cache_append");
   }
   return FFA_OK;
+}
+
+extern "C" int ffa_cache_append_ragged(const void* k, const void* v, int32_t dt, int32_t B, int32_t T_new, int32_t HKV,
+                                       int32_t fp8, uint8_t* base_pool, uint8_t* residual_pool, void* v_pool,
+                                       int32_t n_pages, const int32_t* block_table, int32_t bt_stride, int32_t cols,
+                                       const int32_t* positions, const int32_t* counts, ffa_stream_t stream) {
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (!k || !v || !base_pool || !residual_pool || !v_pool || !block_table || !positions) return FFA_E_NULL;
+  if (B <= 0 || T_new <= 0 || HKV <= 0 || n_pages <= 0 || cols <= 0 || bt_stride < cols) return FFA_E_SHAPE;
+  if ((dt != FFA_F16 && dt != FFA_BF16) || (fp8 != FFA_E5M2 && fp8 != FFA_E4M3)) return FFA_E_DTYPE;
+  if (!aligned16(k) || !aligned16(v) || !aligned16(base_pool) || !aligned16(residual_pool) || !aligned16(v_pool))
+    return FFA_E_ALIGN;
+  const int groups = HKV * D / 8;
+  const int64_t n_vec = static_cast<int64_t>(B) * T_new * groups;
+  int64_t blocks = (n_vec + 255) / 256;
+  if (blocks > 148 * 16) blocks = 148 * 16;
+#define FFA_RAGGED(DT_, F8_)                                                                                     \
+  append_ragged_kernel<DT_, F8_><<<static_cast<unsigned>(blocks), 256, 0, st>>>(                                 \
+      k, static_cast<const uint4*>(v), n_vec, groups, T_new, positions, counts, block_table, bt_stride, cols, n_pages, \
+      base_pool, residual_pool, static_cast<uint4*>(v_pool))
+  if (dt == FFA_BF16) { if (fp8 == FFA_E4M3) FFA_RAGGED(kBF16, kE4M3); else FFA_RAGGED(kBF16, kE5M2); }
+  else { if (fp8 == FFA_E4M3) FFA_RAGGED(kF16, kE4M3); else FFA_RAGGED(kF16, kE5M2); }
+#undef FFA_RAGGED
+  return last_launch("ffa_cache_append_ragged");
 }
 
 extern "C" int ffa_quantize_append(int32_t variant, const void* k, int32_t dt, int32_t B, int32_t T_new, int32_t HKV,

@@ -255,6 +255,69 @@ int ffa_cache_append(int32_t variant, const void* k, const void* v, int32_t dtyp
                      const int32_t* block_table, int32_t bt_stride, int32_t pos0, ffa_stream_t stream);
 
 /*
+ * The same append for sequences of unequal lengths (fp8 base + fp8 residual): token t of sequence b goes to position
+ * positions[b] + t of its row of block_table [B, bt_stride].  positions [B] and counts [B] (optional; at most T_new
+ * each, the tokens past it are padding) are device memory, so a captured call follows them.  Nothing is written for a
+ * token whose position lies outside the table's `cols` columns or on a page outside 0 .. n_pages - 1 (-1 marks an
+ * entry without a page).  Two sequences must not name the same position of the same page.  No counterpart in the
+ * reference, whose batch has one length.
+ */
+int ffa_cache_append_ragged(const void* k, const void* v, int32_t dtype, int32_t B, int32_t T_new, int32_t HKV,
+                            int32_t fp8_format, uint8_t* base_pool, uint8_t* residual_pool, void* v_pool,
+                            int32_t n_pages, const int32_t* block_table, int32_t bt_stride, int32_t cols,
+                            const int32_t* positions, const int32_t* counts, ffa_stream_t stream);
+
+/*
+ * Pages of a cache that several sequences share (no counterpart in the reference, whose cache is one tensor per
+ * layer).  The state is device memory: block_table [max_seqs, bt_stride] (page numbers, -1 = none; `cols` columns are
+ * used), seq_lens [max_seqs] (tokens), refcount [n_pages] (holders of a page, 0 = free), status [1].  A sequence of n
+ * tokens holds the first ceil(n / 64) entries of its row.  All calls read and write the state on the device and may be
+ * captured; they must not overlap one another on the same state.  Lists of sequence numbers are device memory too.
+ * A call whose arguments are wrong (a sequence number out of range, one listed twice where that is not allowed, ...)
+ * changes nothing and sets FFA_PAGES_BAD_ARGUMENT in status; one that runs out of free pages changes nothing and sets
+ * FFA_PAGES_NO_SPACE.  Free pages are handed out lowest number first.
+ */
+enum { FFA_PAGES_BAD_ARGUMENT = 1, FFA_PAGES_NO_SPACE = 2 };
+typedef struct FfaPageTable {
+  int32_t n_pages, max_seqs, cols, bt_stride; /* max_seqs <= 65536                                                */
+  int32_t* block_table;
+  int32_t* seq_lens;
+  int32_t* refcount;
+  int32_t* status;
+  void* scratch;                        /* ffa_pages_scratch_bytes(n_pages, max_seqs); zero before the first call  */
+  size_t scratch_bytes;
+} FfaPageTable;
+/* The tensors whose page p holds page p of the cache (base, residual, V, of every layer): n_pools base addresses
+ * (device array), each tensor [n_pages, 64, token_bytes] with token_bytes (device array) a multiple of 16 and the
+ * address 16-byte aligned.  n_pools = 0: bookkeeping only. */
+typedef struct FfaPagePools {
+  int32_t n_pools;
+  int32_t max_token_bytes;              /* the largest of token_bytes                                              */
+  const uint64_t* bases;
+  const int32_t* token_bytes;
+} FfaPagePools;
+size_t ffa_pages_scratch_bytes(int32_t n_pages, int32_t max_seqs);
+/* Shortens sequences seqs[i] to new_lens[i] tokens (0 ends one); a length above the present one changes nothing.
+ * Pages past the new length lose this holder.  A sequence may be listed twice: the smaller length holds. */
+int ffa_pages_truncate(const FfaPageTable* table, const int32_t* seqs, const int32_t* new_lens, int32_t n,
+                       ffa_stream_t stream);
+/* Gives the empty sequences children[i] the tokens of parents[i]: the same pages, held once more.  No child twice, no
+ * child among the parents. */
+int ffa_pages_fork(const FfaPageTable* table, const int32_t* parents, const int32_t* children, int32_t n,
+                   ffa_stream_t stream);
+/* Makes room for n_new[i] >= 0 more tokens in seqs[i] (no sequence twice): new pages, and where the partly filled
+ * last page has other holders, a page of its own with the same tokens, copied in all pools.  seq_lens grows by
+ * n_new; the caller then writes the tokens.  All or nothing. */
+int ffa_pages_extend(const FfaPageTable* table, const FfaPagePools* pools, const int32_t* seqs, const int32_t* n_new,
+                     int32_t n, ffa_stream_t stream);
+/* Moves live pages into the free ones with lower numbers, so that with L live pages they are 0 .. L-1: the k-th live
+ * page numbered L or above becomes the k-th free page below L.  block_table_out and refcount_out get the state
+ * afterwards; they may be the state itself.  If they are not, the old state stays valid until its pages are used
+ * anew: the moved pages' old contents are not touched. */
+int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* pools, int32_t* block_table_out,
+                      int32_t* refcount_out, ffa_stream_t stream);
+
+/*
  * Fused K projection + bias + RoPE (+ quantise and scatter into the cache).  Replaces
  *   kproj_rope_quantize_{triton,fused}   ffa-q2fp8/fused_kproj_rope_q2fp8.py:427-566 (two GEMM passes there)
  *   kproj_rope_fp4_{triton,fused}        ffa-fp4fp8/fused_kproj_rope_fp4fp8.py:415-522
@@ -299,7 +362,8 @@ size_t ffa_kproj_workspace_bytes(int32_t B, int32_t T, int32_t HKV, int32_t rope
 const char* ffa_last_cuda_error(void);
 /* Library version, bumped when the ABI changes (2: FfaDecodeArgs ends in v_mean; FfaKprojArgs.slot_pos0;
  * 3: ffa_static_scratch_status, every SBS in one launch; 4: ffa_cache_append, ffa_quantize_append;
- * 5: SBS 16 / 32, the ffa_peer_* entry points, ffa_decode_peer). */
+ * 5: SBS 16 / 32, the ffa_peer_* entry points, ffa_decode_peer; 6: ffa_cache_append_ragged, the ffa_pages_* entry
+ * points). */
 int ffa_abi_version(void);
 
 #ifdef __cplusplus
