@@ -67,6 +67,14 @@ class FfaPagePools(C.Structure):
     _fields_ = [("n_pools", C.c_int32), ("max_token_bytes", C.c_int32), ("bases", C.c_void_p), ("token_bytes", C.c_void_p)]
 
 
+class FfaSharedPrefixArgs(C.Structure):
+    _fields_ = ([(name, C.c_int32) for name in ("B", "HQ", "HKV", "head_dim", "n_groups", "n_pages", "cols", "bt_stride", "q_dtype",
+                                                "v_dtype", "fp8_format", "use_residual")] + [("sm_scale", C.c_float)]
+                + [(name, C.c_void_p) for name in ("q", "k_base", "k_residual", "v", "block_table", "seq_lens", "group_start",
+                                                   "prefix_pages", "out", "partial_out", "workspace")]
+                + [("workspace_bytes", C.c_size_t)])
+
+
 class FfaKprojArgs(C.Structure):
     _fields_ = [
         ("variant", C.c_int32),
@@ -140,6 +148,10 @@ def lib() -> C.CDLL:
     L.ffa_pages_compact.argtypes = [table, pools, vp, vp, vp]
     for name in ("ffa_pages_truncate", "ffa_pages_fork", "ffa_pages_extend", "ffa_pages_compact"):
         getattr(L, name).restype = C.c_int
+    L.ffa_shared_prefix_workspace_bytes.argtypes = [i32, i32, i32]
+    L.ffa_shared_prefix_workspace_bytes.restype = C.c_size_t
+    L.ffa_decode_shared_prefix.argtypes = [C.POINTER(FfaSharedPrefixArgs), vp]
+    L.ffa_decode_shared_prefix.restype = C.c_int
     L.ffa_kproj_rope.argtypes = [C.POINTER(FfaKprojArgs), C.c_void_p]
     L.ffa_kproj_rope.restype = C.c_int
     L.ffa_kproj_workspace_bytes.argtypes = [i32, i32, i32, i32]

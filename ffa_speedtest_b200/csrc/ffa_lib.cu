@@ -15,4 +15,4 @@ int note_cuda_error(cudaError_t e, const char* where) {
 }  // namespace ffa
 
 extern "C" const char* ffa_last_cuda_error(void) { return ffa::g_last_error; }
-extern "C" int ffa_abi_version(void) { return 6; }   // 6: ragged append, page bookkeeping
+extern "C" int ffa_abi_version(void) { return 6; }   // 6: ragged append, page bookkeeping, shared-prefix decode

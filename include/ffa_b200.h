@@ -318,6 +318,48 @@ int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* pools, int3
                       int32_t* refcount_out, ffa_stream_t stream);
 
 /*
+ * Decode attention (q_len = 1) for a batch whose sequences fall into groups that share leading pages: the shared pages
+ * of a group are read once for all its sequences, the rest of each sequence for itself.  Every token counts (no
+ * pruning: a shared page is read once anyway, and the pages that some sequence of a group keeps are nearly all).
+ * Sequence b of group g (group_start[g] <= b < group_start[g + 1]) has seq_lens[b] tokens; tokens below
+ * 64 * prefix_pages[g] are in the pages that the table row of the group's FIRST sequence names, the others in those of
+ * its own row.  A sequence shorter than the prefix sees its first seq_lens[b] tokens; one of length 0 gives zeros.  A
+ * sequence outside every group has no shared part.  All of this is device memory and is read by the kernels, so a
+ * captured call follows it.  Entries outside 0 .. n_pages - 1 read as zero keys and values.  The reference has no
+ * counterpart (its sequences share nothing).
+ */
+typedef struct FfaSharedPrefixArgs {
+  int32_t B, HQ, HKV;       /* B <= 16384, HQ / HKV <= 8                                             */
+  int32_t head_dim;         /* 128                                                                  */
+  int32_t n_groups;         /* 1 .. B                                                               */
+  int32_t n_pages;          /* pages of the pools, n_pages * 64 < 2^31                              */
+  int32_t cols, bt_stride;  /* columns of the block table, and from row to row                      */
+  int32_t q_dtype;          /* FFA_F16 | FFA_BF16 | FFA_F32 (rounded to float16); also the output's */
+  int32_t v_dtype;          /* FFA_F16 | FFA_BF16                                                   */
+  int32_t fp8_format;       /* FFA_E5M2 | FFA_E4M3: base and residual                               */
+  int32_t use_residual;     /* 0: K = base                                                          */
+  float sm_scale;
+  const void* q;            /* [B, HQ, 128]                                                         */
+  const void* k_base;       /* [n_pages, 64, HKV, 128] fp8                                          */
+  const void* k_residual;   /* likewise                                                             */
+  const void* v;            /* [n_pages, 64, HKV, 128]                                              */
+  const int32_t* block_table;  /* [B, bt_stride]                                                    */
+  const int32_t* seq_lens;     /* [B]                                                               */
+  const int32_t* group_start;  /* [n_groups + 1], ascending from 0 to B                             */
+  const int32_t* prefix_pages; /* [n_groups]                                                        */
+  void* out;                /* [B, HQ, 128] in q_dtype                                              */
+  float* partial_out;       /* optional [B, HQ, 129] fp32: normalised output and base-2 log-sum-exp
+                               (-inf without a token), as ffa_merge_partials takes them             */
+  void* workspace;          /* ffa_shared_prefix_workspace_bytes(...); its first 512 bytes zero before
+                               the first call.  The int at byte 256 is set when a bounded wait inside
+                               a kernel gave up; the outputs it touched are then NaN.  Calls that share
+                               a workspace must not overlap                                         */
+  size_t workspace_bytes;
+} FfaSharedPrefixArgs;
+size_t ffa_shared_prefix_workspace_bytes(int32_t B, int32_t HQ, int32_t HKV);
+int ffa_decode_shared_prefix(const FfaSharedPrefixArgs* args, ffa_stream_t stream);
+
+/*
  * Fused K projection + bias + RoPE (+ quantise and scatter into the cache).  Replaces
  *   kproj_rope_quantize_{triton,fused}   ffa-q2fp8/fused_kproj_rope_q2fp8.py:427-566 (two GEMM passes there)
  *   kproj_rope_fp4_{triton,fused}        ffa-fp4fp8/fused_kproj_rope_fp4fp8.py:415-522
@@ -363,7 +405,7 @@ const char* ffa_last_cuda_error(void);
 /* Library version, bumped when the ABI changes (2: FfaDecodeArgs ends in v_mean; FfaKprojArgs.slot_pos0;
  * 3: ffa_static_scratch_status, every SBS in one launch; 4: ffa_cache_append, ffa_quantize_append;
  * 5: SBS 16 / 32, the ffa_peer_* entry points, ffa_decode_peer; 6: ffa_cache_append_ragged, the ffa_pages_* entry
- * points). */
+ * points, ffa_decode_shared_prefix). */
 int ffa_abi_version(void);
 
 #ifdef __cplusplus
