@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kPlanThreads) sp_plan_kernel(const __grid_cons
     p.hdr[0] = n_seg;
     p.hdr[1] = n_shared;
     p.hdr[2] = total;
+    p.hdr[3] = 0;
   }
   __syncthreads();
   const int64_t W = static_cast<int64_t>(total) * p.HKV;
@@ -123,79 +124,6 @@ __global__ void __launch_bounds__(kPlanThreads) sp_plan_kernel(const __grid_cons
     p.start[4 * c] = lo;
     p.start[4 * c + 1] = static_cast<int>(in / tiles);
     p.start[4 * c + 2] = static_cast<int>(in % tiles);
-  }
-}
-
-template <int F8>
-__device__ __forceinline__ float4 load_fp8x4(const uint8_t* at) {
-  const uint32_t x = *reinterpret_cast<const uint32_t*>(at);
-  const float2 a = unpack_h2(fp8x2_to_h2<F8>(x)), b = unpack_h2(fp8x2_to_h2<F8>(x >> 16));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-
-// A warp takes query rows one by one and the tokens of the run four at a time; a lane holds four channels.
-template <int F8>
-__global__ void __launch_bounds__(256) sp_attend_kernel(const __grid_constant__ SpParams p) {
-  const int64_t W = static_cast<int64_t>(p.hdr[2]) * p.HKV;
-  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_used = sp_ctas(W, p.n_ctas);
-  if (c >= n_used) return;
-  int64_t left = sp_first(c + 1, W, n_used) - sp_first(c, W, n_used);
-  int si = p.start[4 * c], head = p.start[4 * c + 1], tile = p.start[4 * c + 2];
-  while (left > 0) {
-    const SpSegment s = p.seg[si];
-    if (head >= p.HKV || s.tiles == 0) { ++si; head = 0; tile = 0; continue; }
-    const int n = static_cast<int>(left < s.tiles - tile ? left : s.tiles - tile);
-    const int64_t part = sp_part_row(p, s, head, c);
-    const int32_t* pages = p.bt + static_cast<int64_t>(s.table_row) * p.bt_stride;
-    for (int row = warp; row < s.rows; row += 8) {
-      const int seq = (s.row0 + row) / p.G, g = (s.row0 + row) % p.G;
-      const int64_t qi = (static_cast<int64_t>(seq) * p.HQ + head * p.G + g) * kHeadDim + lane * 4;
-      float q[4], o[4] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = load_as_float(p.q, qi + i, p.q_dtype) * p.scale_log2;
-      const int t0 = s.page0 * kPage + tile * kSpTile;
-      const int t1 = min(min(t0 + n * kSpTile, s.end), p.seq_lens[seq]);
-      for (int t = t0; t < t1; t += 4) {
-        float d[4], w[4];
-        int64_t at[4];
-        float top = m;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int page = t + u < t1 ? pages[(t + u) / kPage] : -1;
-          at[u] = page >= 0 && page < p.n_pages
-                      ? ((static_cast<int64_t>(page) * kPage + (t + u) % kPage) * p.HKV + head) * kHeadDim + lane * 4 : -1;
-          d[u] = 0.f;
-          if (at[u] >= 0) {
-            float4 k = load_fp8x4<F8>(p.k + at[u]);
-            if (p.r) { const float4 r = load_fp8x4<F8>(p.r + at[u]); k.x += r.x; k.y += r.y; k.z += r.z; k.w += r.w; }
-            d[u] = q[0] * k.x + q[1] * k.y + q[2] * k.z + q[3] * k.w;
-          }
-#pragma unroll
-          for (int x = 16; x; x >>= 1) d[u] += __shfl_xor_sync(0xffffffffu, d[u], x);
-          if (t + u >= t1) d[u] = -INFINITY;
-          top = fmaxf(top, d[u]);
-        }
-        const float keep = exp2f(m - top);
-        l *= keep;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= keep;
-        m = top;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          w[u] = exp2f(d[u] - m);
-          l += w[u];
-          if (at[u] >= 0)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] += w[u] * load_as_float(p.v, at[u] + i, p.v_dtype);
-        }
-      }
-      if (lane == 0) p.part_ml[part + row] = make_float2(m, l);
-      *reinterpret_cast<float4*>(p.part_o + (part + row) * kHeadDim + lane * 4) = make_float4(o[0], o[1], o[2], o[3]);
-    }
-    left -= n;
-    tile = 0;
-    ++head;
   }
 }
 
@@ -234,7 +162,7 @@ __global__ void __launch_bounds__(256) sp_merge_kernel(const __grid_constant__ S
       m = top;
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = p.hdr[3] ? NAN : l == 0.f ? 0.f : 1.f / l;      // NaN: a wait of this call gave up
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] *= inv;
 #pragma unroll
@@ -336,9 +264,7 @@ extern "C" int ffa_decode_shared_prefix(const FfaSharedPrefixArgs* a, ffa_stream
   sp_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
   int rc = last_launch("ffa_decode_shared_prefix (plan)");
   if (rc) return rc;
-  if (p.fp8 == FFA_E4M3) sp_attend_kernel<FFA_E4M3><<<p.n_ctas, 256, 0, st>>>(p);
-  else sp_attend_kernel<FFA_E5M2><<<p.n_ctas, 256, 0, st>>>(p);
-  if ((rc = last_launch("ffa_decode_shared_prefix"))) return rc;
+  if ((rc = launch_sp_attend(p, st))) return rc;
   const int64_t rows = static_cast<int64_t>(p.B) * p.HQ;
   sp_merge_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(p);
   return last_launch("ffa_decode_shared_prefix (merge)");

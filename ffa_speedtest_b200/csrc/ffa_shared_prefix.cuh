@@ -43,7 +43,8 @@ struct SpParams {
   float* partial_out;                         // optional [B, HQ, 129]
   int32_t* status;
   // workspace
-  int32_t* hdr;                               // [0] segments, [1] of which shared, [2] tiles of all units of one kv-head
+  int32_t* hdr;                               // [0] segments, [1] of which shared, [2] tiles of all units of one kv-head,
+                                              // [3] a wait of this call gave up
   SpSegment* seg;                             // [max_seg]
   int32_t* cum;                               // [max_seg + 1] tiles of the segments before
   int32_t* start;                             // [n_ctas, 4] segment, kv-head, tile, unused
@@ -77,5 +78,8 @@ __device__ __forceinline__ int sp_ctas(int64_t W, int n_ctas) { return W < 1 ? 1
 // Tiles [c * W / n, (c + 1) * W / n) of all W belong to CTA c; sp_owner is the CTA of tile x.
 __device__ __forceinline__ int64_t sp_first(int64_t c, int64_t W, int n) { return c * W / n; }
 __device__ __forceinline__ int sp_owner(int64_t x, int64_t W, int n) { return static_cast<int>(((x + 1) * n - 1) / W); }
+
+// ffa_shared_prefix_attend.cu: the attention over the runs that the plan in p.hdr, p.seg, ... lists.
+int launch_sp_attend(const SpParams& p, cudaStream_t st);
 
 }  // namespace ffa
