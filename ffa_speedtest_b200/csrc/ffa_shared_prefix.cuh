@@ -3,9 +3,9 @@
 //
 //   o_b = softmax(scale * q_b K_b^T) V_b over the len_b tokens of sequence b,  K = base + residual
 //
-// The batch is cut into segments: one per group of sequences with a shared prefix and 128 of its query rows (a row =
-// one query head of one sequence), holding the group's shared pages; one per sequence, holding its own pages.  A
-// segment and a kv-head make a unit of ceil(tokens / 128) tiles; all units' tiles in a row are cut into equal ranges,
+// The batch is cut into segments: one per sequence, holding its own pages; one per group of sequences with a shared
+// prefix and 128 of its query rows (a row = one query head of one sequence), holding the group's shared pages.  A
+// segment and a kv-head make a unit of ceil(tokens / 128) tiles; all units in a row are cut into ranges of equal cost,
 // one per CTA.  A CTA's part of a unit is a run; every run leaves one partial (maximum, sum, output) per row, and the
 // merge adds a row's partials up in the order of the tiles.  Group sizes, prefix lengths and sequence lengths are read
 // on the device, so a captured call follows them.
@@ -43,17 +43,19 @@ struct SpParams {
   float* partial_out;                         // optional [B, HQ, 129]
   int32_t* status;
   // workspace
-  int32_t* hdr;                               // [0] segments, [1] of which shared, [2] tiles of all units of one kv-head,
-                                              // [3] a wait of this call gave up
-  SpSegment* seg;                             // [max_seg]
-  int32_t* cum;                               // [max_seg + 1] tiles of the segments before
-  int32_t* start;                             // [n_ctas, 4] segment, kv-head, tile, unused
-  int32_t* seq_seg;                           // [B, 2] first segment of the sequence's group (-1: none), its first row
+  int32_t* hdr;                               // [0] segments, [1] cost of all units of one kv-head, [2] a wait of this call gave up
+  SpSegment* seg;                             // [max_seg]: the sequences' own first, then the shared ones
+  int32_t* cum;                               // [max_seg + 1] cost of the segments before
+  int32_t* start;                             // [n_ctas, 2] first segment and kv-head
+  int32_t* seq_seg;                           // [B, 2] first shared segment of the sequence's group (-1: none), its first row
+  uint8_t* qp;                                // [pieces, HKV, B * G, 128] q as e4m3 pieces
+  float* q_scale;                             // [HKV, B * G] what a dot product with them is multiplied with (log2 units)
   float2* part_ml;                            // [part_rows] maximum (log2 units) and sum
   float* part_o;                              // [part_rows, 128]
   int B, NG, HQ, HKV, G;
   int n_pages, cols, bt_stride;
   int n_ctas;
+  int pieces;
   int q_dtype, v_dtype, fp8;
   float scale_log2;
 };
@@ -73,9 +75,13 @@ __device__ __forceinline__ int64_t sp_part_row(const SpParams& p, const SpSegmen
   const int64_t at = static_cast<int64_t>(s.row0) * p.HKV + static_cast<int64_t>(head) * s.rows;
   return s.own ? sp_shared_rows(p.B, p.HQ, p.n_ctas) + at + static_cast<int64_t>(cta) * p.G : at + static_cast<int64_t>(cta) * kSpRows;
 }
-// CTAs that take part: one tile each at least, so that every CTA between a unit's first and last has a run of it.
+
+// A unit costs its tiles and kSpUnitCost for being begun (q, the first loads' latency, the partial).  Its tile t stands at
+// unit_start + kSpUnitCost + t on the line of all costs, 0 .. W; CTA c has [c * W / n, (c + 1) * W / n).
+constexpr int kSpUnitCost = 1;
+__host__ __device__ __forceinline__ int sp_cost(int tiles) { return tiles > 0 ? tiles + kSpUnitCost : 0; }
+// CTAs that take part: one position each at least, so that every CTA between a unit's first and last has a run of it.
 __device__ __forceinline__ int sp_ctas(int64_t W, int n_ctas) { return W < 1 ? 1 : W < n_ctas ? static_cast<int>(W) : n_ctas; }
-// Tiles [c * W / n, (c + 1) * W / n) of all W belong to CTA c; sp_owner is the CTA of tile x.
 __device__ __forceinline__ int64_t sp_first(int64_t c, int64_t W, int n) { return c * W / n; }
 __device__ __forceinline__ int sp_owner(int64_t x, int64_t W, int n) { return static_cast<int>(((x + 1) * n - 1) / W); }
 

@@ -6,25 +6,24 @@
 //   P = 2^(S * row scale - m)                                                           one row per thread
 //   O[128 rows, 128 channels] += P . V                                                  kind::f16, P from TMEM
 //
-// K is used as it lies in the cache: q, scaled by a power of two per row, is split exactly into e4m3 pieces (two hold
-// the 8 significant bits of bf16, three the 11 of fp16), and the products of every piece with the raw base and residual
+// K is used as it lies in the cache: q comes as e4m3 pieces (ffa_shared_prefix.cu), and the products of every piece with the raw base and residual
 // bytes accumulate into one fp32 tile.  That costs 4 (6) fp8 MMAs where a dequantised fp16 K would cost two fp8-MMA
 // times one, but K never passes through registers: TMA writes it, the tensor core reads it.
 //
 // Bound: per 128 tokens and kv-head 64 KiB arrive (about 2800 clocks of an SM's share of HBM); the tensor core needs
 // 4 x 256 + 512 clocks, the softmax warps 128 exponentials per row = 1024 clocks of their SM quarter's unit.
 //
-// Warps: 0 builds the run list and issues TMA; 1 issues MMAs; 2-3 split q; 4-7 softmax (TMEM lanes 32 * (warp % 4)).
+// Warps: 0 builds the run list and loads K and V; 1 issues MMAs; 2 loads q; 4-7 softmax (TMEM lanes 32 * (warp % 4)).
 // A ring of 32 KiB slots holds K tiles (base 16 KiB, residual 16 KiB) and V tiles in the order of use: K0 K1 V0 K2 V1 ...
 // QK of tile i+1 is issued before PV of tile i, so the tensor core works on it while the softmax of tile i runs.  S has
 // two buffers (P overwrites the S it came from), O has two (a run's O is written out while the next run computes).
+// Runs of up to eight query rows (a sequence's own pages) have two small q buffers, larger ones one of 128 rows.
 // MMAs complete in the order of issue, which is what keeps QK(i+2) off the buffer until PV(i) has read P from it.
 //
 // Every wait ends after 0.2 s at most: the CTA then leaves its loops, lets its copies and MMAs in flight finish, and
 // marks the call, and the merge writes NaN.
 #include <cuda.h>
 
-#include "ffa_numeric.h"
 #include "ffa_shared_prefix.cuh"
 
 namespace ffa {
@@ -38,20 +37,21 @@ constexpr unsigned long long kWaitNs = 200ull * 1000 * 1000;
 
 struct Run {
   int32_t table_row, row0, rows, head;
-  int32_t tok0, end, tiles, pad;              // first token, token that ends the segment, tiles
+  int32_t tok0, end, tiles;                   // first token, token that ends the segment, tiles
+  int32_t small;                              // q of at most eight rows
   int64_t part;                               // first row of its partial
 };
 
 template <int NP>                             // pieces of q
 struct Smem {
   static constexpr int kSlots = 5;
-  static constexpr int kOffRing = NP * kPiece;
+  static constexpr int kOffSmall = NP * kPiece;                         // [2][NP] of 8 rows x 128 bytes
+  static constexpr int kOffRing = kOffSmall + 2 * NP * 1024;
   static constexpr int kOffRuns = kOffRing + kSlots * kSlot;
   static constexpr int kOffHead = kOffRuns + 2 * kRunChunk * static_cast<int>(sizeof(Run));   // 2 x (count, last)
-  static constexpr int kOffScale = kOffHead + 16;                       // [4][128] row scales
-  static constexpr int kOffBars = kOffScale + 4 * 128 * 4;
-  // full[slots], empty[slots], sfull[2], pfull[2], odone, ofree[2], qfull, qfree, qscale[4], runfull[2], runempty[2], final
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 1 + 2 + 1 + 1 + 4 + 2 + 2 + 1;
+  static constexpr int kOffBars = kOffHead + 16;
+  // full[slots], empty[slots], sfull[2], pfull[2], odone, ofree[2], qfull[3], qfree[3], runfull[2], runempty[2], final
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 1 + 2 + 3 + 3 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBars + kBars * 8;                 // TMEM address, abort flag, the same for the last waits
   static constexpr int kBytes = kOffMisc + 16 + 1024;                   // and slack to align to 1024
 };
@@ -170,7 +170,9 @@ template <int NP, bool VBF16>
 __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid_constant__ SpParams p,
                                                                     const __grid_constant__ CUtensorMap map_k,
                                                                     const __grid_constant__ CUtensorMap map_r,
-                                                                    const __grid_constant__ CUtensorMap map_v) {
+                                                                    const __grid_constant__ CUtensorMap map_v,
+                                                                    const __grid_constant__ CUtensorMap map_q,
+                                                                    const __grid_constant__ CUtensorMap map_q8) {
   using L = Smem<NP>;
   constexpr int NS = L::kSlots;
   extern __shared__ uint8_t smem_raw[];
@@ -179,7 +181,6 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   const uint32_t s_q = smem_u32(smem), s_ring = s_q + L::kOffRing, bars = s_q + L::kOffBars;
   Run* const runs = reinterpret_cast<Run*>(smem + L::kOffRuns);
   volatile int* const run_head = reinterpret_cast<volatile int*>(smem + L::kOffHead);
-  float* const row_scale = reinterpret_cast<float*>(smem + L::kOffScale);
   volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kOffMisc);
   int* const aborted = reinterpret_cast<int*>(smem + L::kOffMisc + 4);
   auto full = [&](uint32_t s) { return bars + 8 * s; };
@@ -189,15 +190,14 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   auto pfull = [&](uint32_t i) { return rest + 16 + 8 * i; };
   const uint32_t odone = rest + 32;
   auto ofree = [&](uint32_t i) { return rest + 40 + 8 * i; };
-  const uint32_t qfull = rest + 56, qfree = rest + 64;
-  auto qscale = [&](uint32_t i) { return rest + 72 + 8 * i; };
+  // q buffers: 0 the large one, 1 and 2 the small ones
+  auto qfull = [&](uint32_t i) { return rest + 56 + 8 * i; };
+  auto qfree = [&](uint32_t i) { return rest + 80 + 8 * i; };
   auto runfull = [&](uint32_t i) { return rest + 104 + 8 * i; };
   auto runempty = [&](uint32_t i) { return rest + 120 + 8 * i; };
   const uint32_t final_bar = rest + 136;
-
-  const int64_t W = static_cast<int64_t>(p.hdr[2]) * p.HKV;
-  const int n_used = sp_ctas(W, p.n_ctas);
-  if (cta >= n_used || W == 0) return;
+  auto q_buffer = [&](uint32_t i) { return i == 0 ? s_q : s_q + L::kOffSmall + (i - 1) * NP * 1024; };
+  const uint32_t q_piece[2] = {kPiece, 1024};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * NS; ++i) mbar_init(bars + 8 * i, 1);
@@ -206,12 +206,10 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       mbar_init(pfull(i), 4);
       mbar_init(ofree(i), 4);
       mbar_init(runfull(i), 1);
-      mbar_init(runempty(i), 1 + 2 + 4);
+      mbar_init(runempty(i), 1 + 1 + 4);
     }
     mbar_init(odone, 1);
-    mbar_init(qfull, 2);
-    mbar_init(qfree, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(qscale(i), 2);
+    for (int i = 0; i < 3; ++i) { mbar_init(qfull(i), 1); mbar_init(qfree(i), 1); }
     mbar_init(final_bar, 1);
     *aborted = 0;
     aborted[1] = 0;
@@ -225,6 +223,11 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   fence_before();
   __syncthreads();
   fence_after();
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int64_t W = static_cast<int64_t>(p.hdr[1]) * p.HKV;
+  const int n_used = sp_ctas(W, p.n_ctas);
+  const bool idle = cta >= n_used || W == 0;
   const uint32_t tmem = *tmem_slot;           // columns: S0 0, S1 128, O0 256, O1 384
 
   // The next run for a consumer warp, in order; false at the end (or when the CTA gave up).
@@ -251,12 +254,14 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   };
 
   uint32_t issued = 0;                        // warp 0: slots filled so far
-  if (warp == 0) {
-    // ---- run list and TMA ----
+  if (idle) {
+    // nothing for this CTA
+  } else if (warp == 0) {
+    // ---- run list, K and V ----
     const int64_t x0 = sp_first(cta, W, n_used), x1 = sp_first(cta + 1, W, n_used);
     const int n_seg = p.hdr[0];
     const int64_t n_units = static_cast<int64_t>(n_seg) * p.HKV;
-    int64_t unit = static_cast<int64_t>(p.start[4 * cta]) * p.HKV + p.start[4 * cta + 1];
+    int64_t unit = static_cast<int64_t>(p.start[2 * cta]) * p.HKV + p.start[2 * cta + 1];
     // a tile whose V still has to be asked for
     int v_pages[2] = {-1, -1}, v_head = 0, v_n = 0;
     bool have_v = false;
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       if (!past) {
         const int si = static_cast<int>(u / p.HKV), head = static_cast<int>(u % p.HKV);
         const SpSegment s = p.seg[si];
-        const int64_t pos = static_cast<int64_t>(p.cum[si]) * p.HKV + static_cast<int64_t>(head) * s.tiles;
+        const int64_t pos = static_cast<int64_t>(p.cum[si]) * p.HKV + static_cast<int64_t>(head) * sp_cost(s.tiles) + kSpUnitCost;
         past = pos >= x1;
         const int64_t a = pos > x0 ? pos : x0, b = pos + s.tiles < x1 ? pos + s.tiles : x1;
         if (b > a) {
@@ -297,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
           r.tok0 = s.page0 * kPage + static_cast<int>(a - pos) * kSpTile;
           r.end = s.end;
           r.tiles = n;
+          r.small = s.rows <= 8;
           r.part = sp_part_row(p, s, head, cta);
         }
       }
@@ -375,27 +381,32 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     };
     Run r;
     bool ok = true;
+    uint32_t q_large = 0, q_small = 0;        // runs of either kind so far
     while (ok && next_run(r)) {
-      if (!wait(qfull, n_run & 1, aborted)) break;
+      const uint32_t qb = r.small ? 1 + (q_small & 1) : 0;
+      if (!wait(qfull(qb), (r.small ? q_small >> 1 : q_large) & 1, aborted)) break;
+      if (r.small) ++q_small; else ++q_large;
       fence_after();
+      const uint64_t dq = desc(q_buffer(qb), 16);
+      const uint32_t q_step = q_piece[r.small ? 1 : 0] >> 4;
       for (int t = 0; t < r.tiles; ++t) {
         const uint32_t s = used % NS;
         if (!wait(full(s), (used / NS) & 1, aborted)) { ok = false; break; }
         fence_after();
         if (lane == 0) {
-          const uint64_t dk = desc(s_ring + s * kSlot, 16), dq = desc(s_q, 16);
+          const uint64_t dk = desc(s_ring + s * kSlot, 16);
           uint32_t acc = 0;
           for (int part = 0; part < (p.r ? 2 : 1); ++part)
 #pragma unroll
             for (int piece = 0; piece < NP; ++piece)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                mma_fp8(tmem + 128 * (i & 1), dq + (piece * kPiece >> 4) + 2 * k, dk + (part * kPiece >> 4) + 2 * k, idesc_s, acc);
+                mma_fp8(tmem + 128 * (i & 1), dq + piece * q_step + 2 * k, dk + (part * kPiece >> 4) + 2 * k, idesc_s, acc);
                 acc = 1;
               }
           commit(empty(s));
           commit(sfull(i & 1));
-          if (t == r.tiles - 1) commit(qfree);
+          if (t == r.tiles - 1) commit(qfree(qb));
         }
         __syncwarp();
         ++used;
@@ -410,95 +421,25 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       ++n_run;
     }
     if (ok && have && *reinterpret_cast<volatile int*>(aborted) == 0) pv();
-  } else if (warp < 4) {
-    // ---- q: eight lanes to a row, 16 channels to a lane ----
-    int n_run = 0;
+  } else if (warp == 2) {
+    // ---- q ----
+    uint32_t q_large = 0, q_small = 0;
+    const int rows_head = p.B * p.G;
     Run r;
-    const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;
+    asm volatile("fence.proxy.async.global;\n" ::: "memory");       // q's pieces were written by ordinary stores
     while (next_run(r)) {
-      if (n_run > 0 && !wait(qfree, (n_run - 1) & 1, aborted)) break;
-      for (int r0 = (warp - 2) * 4; r0 < r.rows; r0 += 8) {
-        const int row = r0 + (lane >> 3), c0 = (lane & 7) * 16;
-        float x[16];
-        float top = 0.f;
-        if (row < r.rows) {
-          const int seq = (r.row0 + row) / p.G, g = (r.row0 + row) % p.G;
-          const int64_t qi = (static_cast<int64_t>(seq) * p.HQ + r.head * p.G + g) * kHeadDim + c0;
-          if (p.q_dtype == FFA_F32) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qi + 4 * e);
-              x[4 * e] = f.x; x[4 * e + 1] = f.y; x[4 * e + 2] = f.z; x[4 * e + 3] = f.w;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = __half2float(__float2half_rn(x[e]));
-          } else {
-            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + qi);
-            const uint4 a = src[0], b = src[1];
-            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (p.q_dtype == FFA_BF16) {
-                x[2 * e] = __uint_as_float(w[e] << 16);
-                x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-              } else {
-                const float2 f = unpack_h2(w[e]);
-                x[2 * e] = f.x; x[2 * e + 1] = f.y;
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        }
-        bool finite = true;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) { top = fmaxf(top, fabsf(x[e])); finite = finite && fabsf(x[e]) < INFINITY; }
-#pragma unroll
-        for (int d = 4; d; d >>= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          finite = __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, d) && finite;
-        }
-        // 2^up brings the row's largest |q| into [128, 256)
-        const int up = top > 0.f ? min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100) : 0;
-        const float mul = __uint_as_float(static_cast<uint32_t>(up + 127) << 23) * sign;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = finite ? x[e] * mul : 0.f;
-        if (row < r.rows) {
-          if ((lane & 7) == 0)
-            row_scale[(n_run & 3) * 128 + row] =
-                finite ? fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23) : NAN;
-#pragma unroll
-          for (int piece = 0; piece < NP; ++piece) {
-            uint32_t w[4];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              float y[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = x[8 * half + e];
-              const uint2 z = num::narrow8<num::kE4M3>(y);
-              w[2 * half] = z.x; w[2 * half + 1] = z.y;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = num::fp8x2_to_f32x2<num::kE4M3>((e < 2 ? z.x : z.y) >> (16 * (e & 1)));
-                x[8 * half + 2 * e] -= f.x;
-                x[8 * half + 2 * e + 1] -= f.y;
-              }
-            }
-            const uint32_t dst = s_q + piece * kPiece + row * 128 + (((lane & 7) ^ (row & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-          }
-        }
-      }
-      fence_async();
-      __syncwarp();
+      const uint32_t qb = r.small ? 1 + (q_small & 1) : 0, round = r.small ? q_small >> 1 : q_large;
+      if (round > 0 && !wait(qfree(qb), (round - 1) & 1, aborted)) break;
+      if (r.small) ++q_small; else ++q_large;
       if (lane == 0) {
-        mbar_arrive(qscale(n_run & 3));
-        mbar_arrive(qfull);
+        const uint32_t bytes = q_piece[r.small ? 1 : 0];
+        mbar_expect_tx(qfull(qb), NP * bytes);
+        for (int piece = 0; piece < NP; ++piece)
+          tma_load(q_buffer(qb) + piece * bytes, r.small ? &map_q8 : &map_q, 0, (piece * p.HKV + r.head) * rows_head + r.row0, qfull(qb));
       }
-      ++n_run;
+      __syncwarp();
     }
-  } else {
+  } else if (warp >= 4) {
     // ---- softmax: one query row per thread ----
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
@@ -533,9 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       const bool live = row < r.rows, any_live = quarter * 32 < r.rows;
       float m = -INFINITY, l = 0.f, scale = 0.f;
       int end = r.end;
-      if (!wait(qscale(n_run & 3), (n_run >> 2) & 1, aborted)) break;
       if (live) {
-        scale = row_scale[(n_run & 3) * 128 + row];
+        scale = p.q_scale[static_cast<int64_t>(r.head) * p.B * p.G + r.row0 + row];
         end = min(end, p.seq_lens[(r.row0 + row) / p.G]);
       }
       for (int t = 0; t < r.tiles; ++t, ++i) {
@@ -622,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       for (uint32_t n = issued > NS ? issued - NS : 0; n < issued; ++n) {
         wait_lane(full(n % NS), (n / NS) & 1, aborted + 1);
       }
-      if (lane == 0) { p.hdr[3] = 1; atomicExch(p.status, 1); }
+      if (lane == 0) { p.hdr[2] = 1; atomicExch(p.status, 1); }
     } else if (warp == 1) {
       if (lane == 0) commit(final_bar);
       __syncwarp();
@@ -652,11 +592,11 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// Token rows of `row_bytes`; a box is 128 bytes of 64 tokens, 128-byte swizzle.
-bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t row_bytes, CUtensorMapL2promotion promo) {
+// Rows of `row_bytes`; a box is 128 bytes of box_rows of them, 128-byte swizzle.
+bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t row_bytes, uint32_t box_rows, CUtensorMapL2promotion promo) {
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
-  const cuuint32_t box[2] = {128, kPage}, ones[2] = {1, 1};
+  const cuuint32_t box[2] = {128, box_rows}, ones[2] = {1, 1};
   return encode_tiled()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promo,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -672,8 +612,18 @@ int launch(const SpParams& p, const CUtensorMap* maps, cudaStream_t st) {
     if (e != cudaSuccess) return note_cuda_error(e, "cudaFuncSetAttribute(sp_attend_mma)");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  sp_attend_mma_kernel<NP, VBF16><<<p.n_ctas, kThreads, Smem<NP>::kBytes, st>>>(p, maps[0], maps[1], maps[2]);
-  const cudaError_t e = cudaGetLastError();
+  // set up while the plan still runs; it waits for the plan's end before it reads
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.n_ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Smem<NP>::kBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sp_attend_mma_kernel<NP, VBF16>, p, maps[0], maps[1], maps[2], maps[3], maps[4]);
   return e == cudaSuccess ? FFA_OK : note_cuda_error(e, "ffa_decode_shared_prefix");
 }
 
@@ -681,12 +631,15 @@ int launch(const SpParams& p, const CUtensorMap* maps, cudaStream_t st) {
 
 int launch_sp_attend(const SpParams& p, cudaStream_t st) {
   if (!encode_tiled()) return FFA_E_LAUNCH;
-  alignas(64) CUtensorMap maps[3];
+  alignas(64) CUtensorMap maps[5];
   const int64_t rows = static_cast<int64_t>(p.n_pages) * kPage, k_bytes = static_cast<int64_t>(p.HKV) * 128;
+  const int64_t q_rows = static_cast<int64_t>(p.pieces) * p.B * p.HQ;
   // L2 promotion no wider than one head's row: the neighbouring heads belong to other units
-  if (!make_map(&maps[0], p.k, rows, k_bytes, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
-      !make_map(&maps[1], p.r ? p.r : p.k, rows, k_bytes, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
-      !make_map(&maps[2], p.v, rows, 2 * k_bytes, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
+  if (!make_map(&maps[0], p.k, rows, k_bytes, kPage, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
+      !make_map(&maps[1], p.r ? p.r : p.k, rows, k_bytes, kPage, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
+      !make_map(&maps[2], p.v, rows, 2 * k_bytes, kPage, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+      !make_map(&maps[3], p.qp, q_rows, 128, kSpRows, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+      !make_map(&maps[4], p.qp, q_rows, 128, 8, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
     return FFA_E_LAUNCH;
   const bool two = p.q_dtype == FFA_BF16, bf = p.v_dtype == FFA_BF16;
   if (two) return bf ? launch<2, true>(p, maps, st) : launch<2, false>(p, maps, st);

@@ -23,7 +23,7 @@ class SharedPrefixWorkspace:
         self.B, self.HQ, self.HKV, self.device, self.dtype = int(B), int(HQ), int(HKV), torch.device(device), dtype
         nbytes = _lib.lib().ffa_shared_prefix_workspace_bytes(self.B, self.HQ, self.HKV)
         if nbytes == 0:
-            raise ValueError(f"no workspace for B={B}, HQ={HQ}, HKV={HKV}: B must be 1 to 16384, HQ a multiple of HKV")
+            raise ValueError(f"no workspace for B={B}, HQ={HQ}, HKV={HKV}: B must be 1 to 4096, HQ a multiple of HKV")
         self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.scratch[:512].zero_()
         self.o = torch.empty((self.B, self.HQ, 128), dtype=dtype, device=self.device)

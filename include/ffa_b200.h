@@ -329,7 +329,7 @@ int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* pools, int3
  * counterpart (its sequences share nothing).
  */
 typedef struct FfaSharedPrefixArgs {
-  int32_t B, HQ, HKV;       /* B <= 16384, HQ / HKV <= 8                                             */
+  int32_t B, HQ, HKV;       /* B <= 4096, HQ / HKV <= 8                                              */
   int32_t head_dim;         /* 128                                                                  */
   int32_t n_groups;         /* 1 .. B                                                               */
   int32_t n_pages;          /* pages of the pools, n_pages * 64 < 2^31                              */
