@@ -153,6 +153,12 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+// One lane of the converged warp, by the instruction that tells the compiler that it is one.
+__device__ __forceinline__ bool elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -177,7 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   constexpr int NS = L::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+  // uniform for the compiler too: MMAs issued under a branch that it takes for divergent cost 100 clocks and more each
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, cta = blockIdx.x;
   const uint32_t s_q = smem_u32(smem), s_ring = s_q + L::kOffRing, bars = s_q + L::kOffBars;
   Run* const runs = reinterpret_cast<Run*>(smem + L::kOffRuns);
   volatile int* const run_head = reinterpret_cast<volatile int*>(smem + L::kOffHead);
@@ -270,14 +277,14 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       if (round > 0 && !wait(empty(s), (round - 1) & 1, aborted)) return false;
       dst = s_ring + s * kSlot;
       bar = full(s);
-      if (lane == 0) mbar_expect_tx(bar, bytes);
+      if (elect()) mbar_expect_tx(bar, bytes);
       ++issued;
       return true;
     };
     auto load_v = [&]() -> bool {
       uint32_t dst, bar;
       if (!slot_for(v_n * 16384, dst, bar)) return false;
-      if (lane == 0)
+      if (elect())
         for (int i = 0; i < v_n; ++i)
           for (int h = 0; h < 2; ++h)
             tma_load(dst + h * 16384 + i * 8192, &map_v, v_head * 256 + h * 128, v_pages[i] * kPage, bar);
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
           const int pg0 = __shfl_sync(0xffffffffu, ids, (2 * t) & 31), pg1 = __shfl_sync(0xffffffffu, ids, (2 * t + 1) & 31);
           uint32_t dst, bar;
           if (!slot_for(n_pages * (p.r ? 16384 : 8192), dst, bar)) { ok = false; break; }
-          if (lane == 0)
+          if (elect())
             for (int i = 0; i < n_pages; ++i) {
               const int y = (i ? pg1 : pg0) * kPage;
               tma_load(dst + i * 8192, &map_k, q.head * 128, y, bar);
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       if (first && o_round > 0 && !wait(ofree(o_buf), (o_round - 1) & 1, aborted)) return false;
       if (!wait(pfull(j & 1), (j >> 1) & 1, aborted)) return false;
       fence_after();
-      if (lane == 0) {
+      if (elect()) {
         const uint64_t dv = desc(v, 16384);
         for (int k = 0; k < steps; ++k)
           mma_16_tmem(tmem + 256 + 128 * o_buf, tmem + 128 * (j & 1) + 8 * k, dv + 128 * k, idesc_o, !(first && k == 0));
@@ -393,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
         const uint32_t s = used % NS;
         if (!wait(full(s), (used / NS) & 1, aborted)) { ok = false; break; }
         fence_after();
-        if (lane == 0) {
+        if (elect()) {
           const uint64_t dk = desc(s_ring + s * kSlot, 16);
           uint32_t acc = 0;
           for (int part = 0; part < (p.r ? 2 : 1); ++part)
@@ -431,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       const uint32_t qb = r.small ? 1 + (q_small & 1) : 0, round = r.small ? q_small >> 1 : q_large;
       if (round > 0 && !wait(qfree(qb), (round - 1) & 1, aborted)) break;
       if (r.small) ++q_small; else ++q_large;
-      if (lane == 0) {
+      if (elect()) {
         const uint32_t bytes = q_piece[r.small ? 1 : 0];
         mbar_expect_tx(qfull(qb), NP * bytes);
         for (int piece = 0; piece < NP; ++piece)
