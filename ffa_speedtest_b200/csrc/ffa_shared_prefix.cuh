@@ -3,12 +3,12 @@
 //
 //   o_b = softmax(scale * q_b K_b^T) V_b over the len_b tokens of sequence b,  K = base + residual
 //
-// The batch is cut into segments: one per sequence, holding its own pages; one per group of sequences with a shared
-// prefix and 128 of its query rows (a row = one query head of one sequence), holding the group's shared pages.  A
-// segment and a kv-head make a unit of ceil(tokens / 128) tiles; all units in a row are cut into ranges of equal cost,
-// one per CTA.  A CTA's part of a unit is a run; every run leaves one partial (maximum, sum, output) per row, and the
-// merge adds a row's partials up in the order of the tiles.  Group sizes, prefix lengths and sequence lengths are read
-// on the device, so a captured call follows them.
+// Items of work: one per sequence (its own pages) and one per group of sequences with a shared prefix (the group's
+// pages, all query rows of the group; a row = one query head of one sequence).  An item is cut into units: a kv-head,
+// and for groups a block of 128 rows.  A unit has ceil(tokens / 128) tiles.  All units stand in a row on a line of costs,
+// which is cut into equal ranges, one per CTA.  A CTA's part of a unit is a run; every run leaves partials (maximum, sum,
+// output) for its rows, and the merge adds a row's partials up in the order of the line.  Group sizes, prefix lengths and
+// sequence lengths are read on the device, so a captured call follows them; every CTA works out the line for itself.
 #pragma once
 
 #include "ffa_common.cuh"
@@ -16,18 +16,21 @@
 namespace ffa {
 
 constexpr int kSpTile = 128;                  // tokens of a tile: two pages
-constexpr int kSpRows = 128;                  // query rows of a segment
+constexpr int kSpRows = 128;                  // query rows of a unit, at most
+constexpr int kSpMaxCtas = 148;
 
-// one segment of the work list
-struct SpSegment {
-  int32_t table_row;                          // row of the block table that names its pages
-  int32_t row0;                               // first query row: sequence * G + head within the group
-  int32_t rows;                               // query rows
-  int32_t tiles;
-  int32_t page0;                              // first column of the block table
-  int32_t end;                                // token position (in the sequence) that ends it
-  int32_t own;                                // 0: shared pages of a group, 1: a sequence's own pages
-  int32_t pad;
+// Costs, in quarters of a tile: beginning a unit (q, the first loads' latency, its partials), and a tile.
+constexpr int kSpBegin = 4, kSpTileCost = 4;
+
+// where the merge finds the partials of a sequence's rows: the places of its item and of its group's on the line
+struct SpSequence {
+  int32_t at, tiles;
+  int32_t group_at, group_tiles;              // 0 tiles: no shared part
+  int32_t group_first, group_rows;            // first sequence of the group, rows of a kv-head
+  int32_t pad[2];
+};
+struct SpGroup {
+  int32_t at, tiles, first, rows;
 };
 
 struct SpParams {
@@ -43,15 +46,13 @@ struct SpParams {
   float* partial_out;                         // optional [B, HQ, 129]
   int32_t* status;
   // workspace
-  int32_t* hdr;                               // [0] segments, [1] cost of all units of one kv-head, [2] a wait of this call gave up
-  SpSegment* seg;                             // [max_seg]: the sequences' own first, then the shared ones
-  int32_t* cum;                               // [max_seg + 1] cost of the segments before
-  int32_t* start;                             // [n_ctas, 2] first segment and kv-head
-  int32_t* seq_seg;                           // [B, 2] first shared segment of the sequence's group (-1: none), its first row
+  int32_t* hdr;                               // [0] length of the line, [1] a wait of this call gave up
+  SpSequence* sequences;                      // [B]
+  SpGroup* groups;                            // [NG]
   uint8_t* qp;                                // [pieces, HKV, B * G, 128] q as e4m3 pieces
   float* q_scale;                             // [HKV, B * G] what a dot product with them is multiplied with (log2 units)
   float2* part_ml;                            // [part_rows] maximum (log2 units) and sum
-  float* part_o;                              // [part_rows, 128]
+  float4* part_o;                             // [part_rows, 32]
   int B, NG, HQ, HKV, G;
   int n_pages, cols, bt_stride;
   int n_ctas;
@@ -60,32 +61,96 @@ struct SpParams {
   float scale_log2;
 };
 
-// Segments of shared pages: every group begins one, and one more for every 128 rows (at most B groups).
-__host__ __device__ inline int64_t sp_max_shared(int64_t B, int64_t G) { return B + B * G / kSpRows + 1; }
-
-// Rows of partials: a run of CTA c in unit (segment, kv-head) writes at
-//   shared: row0 * HKV + head * rows + c * 128        (rows before it in the unit order, plus 128 for each CTA before)
+// Rows of partials.  A run of CTA c in the unit of these rows and this head begins at
+//   shared: row0 * HKV + head * rows + c * 128        (rows before it in the order of the line, plus 128 for each CTA before)
 //   own:    shared_rows + row0 * HKV + head * G + c * G
-// Going on to the next unit or the next CTA moves at least `rows` rows on, so no two runs share a row.
-__host__ __device__ inline int64_t sp_shared_rows(int64_t B, int64_t HQ, int64_t n_ctas) { return B * HQ + n_ctas * kSpRows; }
-__host__ __device__ inline int64_t sp_part_rows(int64_t B, int64_t HQ, int64_t HKV, int64_t n_ctas) {
-  return sp_shared_rows(B, HQ, n_ctas) + B * HQ + n_ctas * (HQ / HKV);
+// Going on to the next unit or the next CTA moves at least `rows` rows on, so no two runs share a row.  With `at` the run's
+// first row, row j's partial is part_ml[at + j], and its channels 4 * c .. 4 * c + 3 are part_o[32 * at + c * rows + j], so
+// that the threads that hold a row each write side by side.
+__host__ __device__ inline int64_t sp_shared_rows(int64_t B, int64_t HQ) { return B * HQ + static_cast<int64_t>(kSpMaxCtas) * kSpRows; }
+__host__ __device__ inline int64_t sp_part_rows(int64_t B, int64_t HQ, int64_t HKV) {
+  return sp_shared_rows(B, HQ) + B * HQ + kSpMaxCtas * (HQ / HKV);
 }
-__device__ __forceinline__ int64_t sp_part_row(const SpParams& p, const SpSegment& s, int head, int cta) {
-  const int64_t at = static_cast<int64_t>(s.row0) * p.HKV + static_cast<int64_t>(head) * s.rows;
-  return s.own ? sp_shared_rows(p.B, p.HQ, p.n_ctas) + at + static_cast<int64_t>(cta) * p.G : at + static_cast<int64_t>(cta) * kSpRows;
+__device__ __forceinline__ int64_t sp_part_row(const SpParams& p, bool own, int row0, int rows, int head, int cta) {
+  const int64_t at = static_cast<int64_t>(row0) * p.HKV + static_cast<int64_t>(head) * rows;
+  return own ? sp_shared_rows(p.B, p.HQ) + at + static_cast<int64_t>(cta) * p.G : at + static_cast<int64_t>(cta) * kSpRows;
 }
 
-// A unit costs its tiles and kSpUnitCost for being begun (q, the first loads' latency, the partial).  Its tile t stands at
-// unit_start + kSpUnitCost + t on the line of all costs, 0 .. W; CTA c has [c * W / n, (c + 1) * W / n).
-constexpr int kSpUnitCost = 1;
-__host__ __device__ __forceinline__ int sp_cost(int tiles) { return tiles > 0 ? tiles + kSpUnitCost : 0; }
-// CTAs that take part: one position each at least, so that every CTA between a unit's first and last has a run of it.
-__device__ __forceinline__ int sp_ctas(int64_t W, int n_ctas) { return W < 1 ? 1 : W < n_ctas ? static_cast<int>(W) : n_ctas; }
-__device__ __forceinline__ int64_t sp_first(int64_t c, int64_t W, int n) { return c * W / n; }
-__device__ __forceinline__ int sp_owner(int64_t x, int64_t W, int n) { return static_cast<int>(((x + 1) * n - 1) / W); }
+// Cost of a unit of so many tiles.  Tile t of a unit that begins at U stands at U + kSpBegin + t * kSpTileCost.
+__device__ __forceinline__ int sp_unit_cost(int tiles) { return tiles > 0 ? kSpBegin + tiles * kSpTileCost : 0; }
+// The line is at most this long (the host refuses what could give 2^31 or more).
+__host__ __device__ inline int64_t sp_longest_line(int64_t B, int64_t NG, int64_t HKV, int64_t G, int64_t cols) {
+  return HKV * (kSpBegin + (cols + 1) / 2 * kSpTileCost) * (B + NG + B * G / kSpRows);
+}
+// CTAs that take part on a line of length W: each gets 4 at least, a tile, so that every CTA between the first and the
+// last of a unit has a tile of it (8 on average, less what rounding takes).  CTA c begins at c * (W / n).
+__device__ __forceinline__ int sp_ctas(int W, int n_ctas) { return max(1, min(n_ctas, W / 8)); }
+__device__ __forceinline__ int sp_first(int c, int W, int n) {
+  return c >= n ? W : static_cast<int>(static_cast<float>(c) * (static_cast<float>(W) * __frcp_rn(static_cast<float>(n))));
+}
+__device__ __forceinline__ int sp_owner(int x, int W, int n) {
+  int c = min(n - 1, static_cast<int>(static_cast<float>(x) * (static_cast<float>(n) * __frcp_rn(static_cast<float>(W)))));
+  while (c > 0 && sp_first(c, W, n) > x) --c;
+  while (c < n - 1 && sp_first(c + 1, W, n) <= x) ++c;
+  return c;
+}
 
-// ffa_shared_prefix_attend.cu: the attention over the runs that the plan in p.hdr, p.seg, ... lists.
+// Lengths and group bounds come from the caller's device memory and are clamped to the batch and the table, so that
+// whatever they hold no access leaves the tensors.
+// Group bounds and prefixes, clamped: in the CTA's shared memory as far as they fit there.  Bounds that do not ascend make
+// no groups at all (n = 0), so that a row never belongs to two.
+constexpr int kSpGroupsNear = 256;
+struct SpBounds {
+  const SpParams& p;
+  int n;                                      // groups
+  const int32_t* near_start;                  // [min(NG, kSpGroupsNear) + 1]
+  const int32_t* near_pages;
+  __device__ __forceinline__ int start(int g) const {
+    return g <= kSpGroupsNear ? near_start[g] : min(max(p.group_start[g], 0), p.B);
+  }
+  __device__ __forceinline__ int pages(int g) const { return g < kSpGroupsNear ? near_pages[g] : min(max(p.prefix_pages[g], 0), p.cols); }
+  // the group of sequence b, or -1
+  __device__ __forceinline__ int group_of(int b) const {
+    int lo = 0, hi = n;                       // last group that starts at or before b
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (start(mid) <= b) lo = mid + 1; else hi = mid;
+    }
+    return lo > 0 && b < start(lo) ? lo - 1 : -1;
+  }
+};
+
+// Item i of the line: sequences 0 .. B-1 (len: seq_lens[i]), then groups.
+struct SpItem {
+  int first, rows;                            // first sequence (its table row), rows of a kv-head, all blocks
+  int page0, end, tiles;                      // first column of the block table, token that ends it
+  int units;
+  int group;                                  // of a sequence: its group
+};
+__device__ __forceinline__ SpItem sp_item(const SpParams& p, const SpBounds& bounds, int i, int len) {
+  SpItem x;
+  if (i < p.B) {
+    x.group = bounds.group_of(i);
+    x.first = i;
+    x.rows = p.G;
+    x.page0 = x.group >= 0 ? bounds.pages(x.group) : 0;
+    x.end = min(max(len, 0), p.cols * kPage);
+    x.tiles = (max(x.end - x.page0 * kPage, 0) + kSpTile - 1) / kSpTile;
+    x.units = p.HKV;
+  } else {
+    const int g = i - p.B;
+    x.group = -1;
+    x.first = bounds.start(g);
+    x.rows = (bounds.start(g + 1) - x.first) * p.G;
+    x.page0 = 0;
+    x.end = x.rows ? bounds.pages(g) * kPage : 0;
+    x.tiles = (x.end + kSpTile - 1) / kSpTile;
+    x.units = (x.rows + kSpRows - 1) / kSpRows * p.HKV;
+  }
+  return x;
+}
+
+// ffa_shared_prefix_attend.cu: the attention over the runs; it also leaves what the merge has to know of the line.
 int launch_sp_attend(const SpParams& p, cudaStream_t st);
 
 }  // namespace ffa

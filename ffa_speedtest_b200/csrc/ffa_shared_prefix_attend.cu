@@ -1,24 +1,28 @@
 // Attention over the runs of the shared-prefix decode (ffa_shared_prefix.cuh) on the fifth-generation tensor cores.
 //
-// One persistent CTA per SM walks its runs tile by tile (128 query rows x 128 tokens):
+// One persistent CTA per SM walks its runs in steps of 128 query rows x 128 tokens:
 //
 //   S[128 rows, 128 tokens] = sum over pieces of q, base and residual:  Qpiece . K^T    kind::f8f6f4, fp32 in TMEM
 //   P = 2^(S * row scale - m)                                                           one row per thread
 //   O[128 rows, 128 channels] += P . V                                                  kind::f16, P from TMEM
 //
-// K is used as it lies in the cache: q comes as e4m3 pieces (ffa_shared_prefix.cu), and the products of every piece with the raw base and residual
-// bytes accumulate into one fp32 tile.  That costs 4 (6) fp8 MMAs where a dequantised fp16 K would cost two fp8-MMA
-// times one, but K never passes through registers: TMA writes it, the tensor core reads it.
+// K is used as it lies in the cache: q comes as e4m3 pieces (ffa_shared_prefix.cu), and the products of every piece with
+// the raw base and residual bytes accumulate into one fp32 tile.  That costs 4 (6) times the fp8 MMAs of one product,
+// twice (three times) what a dequantised 16-bit K would, but K never passes through registers.
 //
-// Bound: per 128 tokens and kv-head 64 KiB arrive (about 2800 clocks of an SM's share of HBM); the tensor core needs
-// 4 x 256 + 512 clocks, the softmax warps 128 exponentials per row = 1024 clocks of their SM quarter's unit.
+// Bound: per 128 tokens and kv-head 64 KiB arrive, 2840 clocks of an SM's share of HBM at 1.9 GHz.  The tensor core needs
+// 16 (24) + 8 MMAs of 64 clocks a step.  The softmax of a row takes 128 exponentials, 1024 clocks of the special-function
+// unit of a quarter of the SM, and some 1000 clocks around them (exponentials by a polynomial on the FMA units were tried:
+// half of them so made a step 600 clocks longer).
 //
-// Warps: 0 builds the run list and loads K and V; 1 issues MMAs; 2 loads q; 4-7 softmax (TMEM lanes 32 * (warp % 4)).
-// A ring of 32 KiB slots holds K tiles (base 16 KiB, residual 16 KiB) and V tiles in the order of use: K0 K1 V0 K2 V1 ...
-// QK of tile i+1 is issued before PV of tile i, so the tensor core works on it while the softmax of tile i runs.  S has
-// two buffers (P overwrites the S it came from), O has two (a run's O is written out while the next run computes).
-// Runs of up to eight query rows (a sequence's own pages) have two small q buffers, larger ones one of 128 rows.
-// MMAs complete in the order of issue, which is what keeps QK(i+2) off the buffer until PV(i) has read P from it.
+// Warps: 0 lists the runs and loads q, K and V; 1 issues the MMAs of S, 2 those of O (two warps, so that the waits of one
+// do not keep the other's from the tensor core); 4-7 softmax (TMEM lanes 32 * (warp % 4)).
+// A ring of 16 KiB slots holds, tile after tile, K base, K residual, V of the first and of the second page.  S has two
+// buffers, for even and odd steps: S of step i+1 is made while the softmax of step i runs.  P overwrites the S that it came
+// from.  O has two buffers, for even and odd runs: a run's O is written out while the next run has begun.
+// Runs of up to eight query rows (a sequence's own pages) have two small q buffers, larger ones one of 256 rows.
+//
+// The line of costs does not depend on the kernel that splits q, nor do K and V: both are begun while that one runs.
 //
 // Every wait ends after 0.2 s at most: the CTA then leaves its loops, lets its copies and MMAs in flight finish, and
 // marks the call, and the merge writes NaN.
@@ -30,32 +34,36 @@ namespace ffa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSlot = 32 * 1024;
+constexpr int kSlot = 16 * 1024;
 constexpr int kPiece = 16 * 1024;             // 128 rows x 128 bytes
-constexpr int kRunChunk = 32;
+constexpr int kRuns = 8;                      // runs listed ahead
 constexpr unsigned long long kWaitNs = 200ull * 1000 * 1000;
 
 struct Run {
   int32_t table_row, row0, rows, head;
-  int32_t tok0, end, tiles;                   // first token, token that ends the segment, tiles
-  int32_t small;                              // q of at most eight rows
-  int64_t part;                               // first row of its partial
+  int32_t tok0, end, tiles;                   // first token, token that ends the item, tiles (0: no more runs)
+  int32_t small;                              // up to eight query rows
+  int64_t part;                               // first row of its partials
 };
 
 template <int NP>                             // pieces of q
 struct Smem {
-  static constexpr int kSlots = 5;
-  static constexpr int kOffSmall = NP * kPiece;                         // [2][NP] of 8 rows x 128 bytes
+  static constexpr int kSlots = NP == 2 ? 11 : 10;
+  static constexpr int kOffSmall = NP * kPiece;                         // after [NP] of 128 rows: [2][NP] of 8 rows
   static constexpr int kOffRing = kOffSmall + 2 * NP * 1024;
   static constexpr int kOffRuns = kOffRing + kSlots * kSlot;
-  static constexpr int kOffHead = kOffRuns + 2 * kRunChunk * static_cast<int>(sizeof(Run));   // 2 x (count, last)
-  static constexpr int kOffBars = kOffHead + 16;
-  // full[slots], empty[slots], sfull[2], pfull[2], odone, ofree[2], qfull[3], qfree[3], runfull[2], runempty[2], final
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 1 + 2 + 3 + 3 + 2 + 2 + 1;
+  static constexpr int kOffPlan = kOffRuns + kRuns * static_cast<int>(sizeof(Run));    // [12] sums of the warps; [12], [13] first item, its place; the item
+  static constexpr int kOffBounds = kOffPlan + 64 + 48;                     // group bounds and prefixes
+  static constexpr int kOffBars = kOffBounds + (2 * kSpGroupsNear + 2) * 4;
+  // full[slots], empty[slots], sfull[2], sfree[2], pfull[2], ofree[2], qfull[3], qfree[3], runfull[runs], runempty[runs],
+  // final[2]
+  static constexpr int kBars = 2 * kSlots + 8 + 6 + 2 * kRuns + 2;
   static constexpr int kOffMisc = kOffBars + kBars * 8;                 // TMEM address, abort flag, the same for the last waits
   static constexpr int kBytes = kOffMisc + 16 + 1024;                   // and slack to align to 1024
 };
 static_assert(Smem<2>::kBytes <= 227 * 1024 && Smem<3>::kBytes <= 227 * 1024, "shared memory of a CTA");
+// K of two tiles and V of one have to fit, or the ring could fill up with what is not needed next
+static_assert(Smem<3>::kSlots >= 6, "slots of the ring");
 
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
@@ -97,6 +105,13 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
 
@@ -148,6 +163,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t* r, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
@@ -164,12 +193,54 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
+// two at a time: a * s + t, a + b
+__device__ __forceinline__ float2 fma2(float2 a, float s, float t) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %5};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(s), "f"(t));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {       // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
   if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// Sum over the CTA's threads before this one; `total` gets the sum over all.  s: one entry per warp.
+__device__ __forceinline__ int cta_exclusive(int x, volatile int* s, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += y;
+  }
+  __syncthreads();
+  if (lane == 31) s[warp] = inc;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int y = s[w];
+    if (w < warp) before += y;
+    total += y;
+  }
+  return before + inc - x;
 }
 
 template <int NP, bool VBF16>
@@ -180,44 +251,59 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
                                                                     const __grid_constant__ CUtensorMap map_q,
                                                                     const __grid_constant__ CUtensorMap map_q8) {
   using L = Smem<NP>;
-  constexpr int NS = L::kSlots;
+  constexpr uint32_t NS = L::kSlots;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   // uniform for the compiler too: MMAs issued under a branch that it takes for divergent cost 100 clocks and more each
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, cta = blockIdx.x;
   const uint32_t s_q = smem_u32(smem), s_ring = s_q + L::kOffRing, bars = s_q + L::kOffBars;
   Run* const runs = reinterpret_cast<Run*>(smem + L::kOffRuns);
-  volatile int* const run_head = reinterpret_cast<volatile int*>(smem + L::kOffHead);
+  volatile int* const s_plan = reinterpret_cast<volatile int*>(smem + L::kOffPlan);
+  SpItem* const s_first = reinterpret_cast<SpItem*>(smem + L::kOffPlan + 64);
+  int* const s_bounds = reinterpret_cast<int*>(smem + L::kOffBounds);
   volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kOffMisc);
   int* const aborted = reinterpret_cast<int*>(smem + L::kOffMisc + 4);
   auto full = [&](uint32_t s) { return bars + 8 * s; };
   auto empty = [&](uint32_t s) { return bars + 8 * (NS + s); };
   const uint32_t rest = bars + 16 * NS;
   auto sfull = [&](uint32_t i) { return rest + 8 * i; };
-  auto pfull = [&](uint32_t i) { return rest + 16 + 8 * i; };
-  const uint32_t odone = rest + 32;
-  auto ofree = [&](uint32_t i) { return rest + 40 + 8 * i; };
+  auto sfree = [&](uint32_t i) { return rest + 16 + 8 * i; };
+  auto pfull = [&](uint32_t i) { return rest + 32 + 8 * i; };
+  auto ofree = [&](uint32_t i) { return rest + 48 + 8 * i; };
   // q buffers: 0 the large one, 1 and 2 the small ones
-  auto qfull = [&](uint32_t i) { return rest + 56 + 8 * i; };
-  auto qfree = [&](uint32_t i) { return rest + 80 + 8 * i; };
-  auto runfull = [&](uint32_t i) { return rest + 104 + 8 * i; };
-  auto runempty = [&](uint32_t i) { return rest + 120 + 8 * i; };
-  const uint32_t final_bar = rest + 136;
+  auto qfull = [&](uint32_t i) { return rest + 64 + 8 * i; };
+  auto qfree = [&](uint32_t i) { return rest + 88 + 8 * i; };
+  auto final_bar = [&](uint32_t i) { return rest + 112 + 8 * i; };
+  auto runfull = [&](uint32_t i) { return rest + 128 + 8 * i; };
+  auto runempty = [&](uint32_t i) { return rest + 128 + 8 * (kRuns + i); };
   auto q_buffer = [&](uint32_t i) { return i == 0 ? s_q : s_q + L::kOffSmall + (i - 1) * NP * 1024; };
-  const uint32_t q_piece[2] = {kPiece, 1024};
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2 * NS; ++i) mbar_init(bars + 8 * i, 1);
+  // what the line is worked out from, on its way before anything else
+  const int tid = threadIdx.x;
+  const int first_len = tid < p.B ? p.seq_lens[tid] : 0;
+  {
+    // the block table into L2, a line to a thread: its entries are asked for once the line is known
+    const int64_t at = (static_cast<int64_t>(cta) * kThreads + tid) * 32;
+    if (at < static_cast<int64_t>(p.B - 1) * p.bt_stride + p.cols) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(p.bt + at));
+  }
+  bool falls = false;                         // a bound below the one before it
+  for (int g = tid; g <= p.NG; g += kThreads) {
+    const int start = p.group_start[g];
+    falls |= g < p.NG && p.group_start[g + 1] < start;
+    if (g <= kSpGroupsNear) s_bounds[g] = min(max(start, 0), p.B);
+    if (g < min(p.NG, kSpGroupsNear)) s_bounds[kSpGroupsNear + 1 + g] = min(max(p.prefix_pages[g], 0), p.cols);
+  }
+  if (warp == 2 && lane == 0) {
+    for (uint32_t i = 0; i < 2 * NS; ++i) mbar_init(bars + 8 * i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull(i), 1);
+      mbar_init(sfree(i), 1);
       mbar_init(pfull(i), 4);
       mbar_init(ofree(i), 4);
-      mbar_init(runfull(i), 1);
-      mbar_init(runempty(i), 1 + 1 + 4);
+      mbar_init(final_bar(i), 1);
     }
-    mbar_init(odone, 1);
+    for (int i = 0; i < kRuns; ++i) { mbar_init(runfull(i), 1); mbar_init(runempty(i), 1 + 1 + 4); }
     for (int i = 0; i < 3; ++i) { mbar_init(qfull(i), 1); mbar_init(qfree(i), 1); }
-    mbar_init(final_bar, 1);
     *aborted = 0;
     aborted[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -227,256 +313,334 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(s_q + L::kOffMisc) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  const int n_groups = __syncthreads_or(falls) ? 0 : p.NG, n_items = p.B + n_groups;
+
+  // ---- the line: its length, and the item that this CTA's range begins in ----
+  const SpBounds bounds{p, n_groups, s_bounds, s_bounds + kSpGroupsNear + 1};
+  SpItem mine{};
+  int W = 0, my_cost = 0, my_at = 0, first_sum = 0;
+  for (int i0 = 0; i0 < n_items; i0 += kThreads) {
+    const int i = i0 + tid;
+    SpItem x{};
+    if (i < n_items) x = sp_item(p, bounds, i, i0 == 0 ? first_len : i < p.B ? p.seq_lens[i] : 0);
+    const int cost = x.units * sp_unit_cost(x.tiles);
+    int sum;
+    const int at = W + cta_exclusive(cost, s_plan, sum);
+    if (i0 == 0) { mine = x; my_cost = cost; my_at = at; first_sum = sum; }
+    if (cta == 0 && i < n_items) {            // for the merge
+      if (i < p.B) p.sequences[i] = SpSequence{at, x.tiles, x.group, 0, 0, 0, {0, 0}};
+      else p.groups[i - p.B] = SpGroup{at, x.tiles, x.first, x.rows};
+    }
+    W += sum;
+  }
+  if (cta == 0 && tid == 0) p.hdr[0] = W;
+  const int n_used = sp_ctas(W, p.n_ctas);
+  const bool idle = cta >= n_used || W == 0;
+  const int x0 = sp_first(cta, W, n_used), x1 = sp_first(cta + 1, W, n_used);
+  if (!idle) {
+    if (my_cost > 0 && my_at <= x0 && x0 < my_at + my_cost) { *s_first = mine; s_plan[12] = tid; s_plan[13] = my_at; }
+    int before = first_sum;
+    for (int i0 = kThreads; i0 < n_items && before <= x0; i0 += kThreads) {
+      const int i = i0 + tid;
+      SpItem x{};
+      if (i < n_items) x = sp_item(p, bounds, i, i < p.B ? p.seq_lens[i] : 0);
+      const int cost = x.units * sp_unit_cost(x.tiles);
+      int sum;
+      const int at = before + cta_exclusive(cost, s_plan, sum);
+      before += sum;
+      if (cost > 0 && at <= x0 && x0 < at + cost) { *s_first = x; s_plan[12] = i; s_plan[13] = at; }
+    }
+  }
   fence_before();
   __syncthreads();
   fence_after();
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int64_t W = static_cast<int64_t>(p.hdr[1]) * p.HKV;
-  const int n_used = sp_ctas(W, p.n_ctas);
-  const bool idle = cta >= n_used || W == 0;
   const uint32_t tmem = *tmem_slot;           // columns: S0 0, S1 128, O0 256, O1 384
 
-  // The next run for a consumer warp, in order; false at the end (or when the CTA gave up).
-  int ch = 0, at = 0, count = -1, last = 0;
-  auto next_run = [&](Run& r) -> bool {
-    for (;;) {
-      if (count < 0) {
-        if (!wait(runfull(ch & 1), (ch >> 1) & 1, aborted)) return false;
-        count = run_head[2 * (ch & 1)];
-        last = run_head[2 * (ch & 1) + 1];
-        at = 0;
-      }
-      if (at < count) {
-        r = runs[(ch & 1) * kRunChunk + at];
-        ++at;
-        return true;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(runempty(ch & 1));
-      if (last) return false;
-      ++ch;
-      count = -1;
+  if (cta == 0 && warp >= 4) {                // these warps have nothing to do yet
+    for (int b = tid - 128; b < p.B; b += kThreads - 128) {
+      const int g = p.sequences[b].group_at;  // the group's number so far
+      const SpGroup gr = g >= 0 ? p.groups[g] : SpGroup{0, 0, 0, 0};
+      p.sequences[b].group_at = gr.at;
+      p.sequences[b].group_tiles = gr.tiles;
+      p.sequences[b].group_first = gr.first;
+      p.sequences[b].group_rows = gr.rows;
     }
+  }
+
+  // The next run for a consumer warp, in order; false at the end (or when the CTA gave up).
+  uint32_t runs_read = 0;
+  auto next_run = [&](Run& r) -> bool {
+    const uint32_t i = runs_read % kRuns;
+    if (!wait(runfull(i), (runs_read / kRuns) & 1, aborted)) return false;
+    r = runs[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(runempty(i));
+    ++runs_read;
+    return r.tiles > 0;
   };
 
+  const uint32_t nk = p.r ? 2 : 1;            // slots of a K tile
   uint32_t issued = 0;                        // warp 0: slots filled so far
   if (idle) {
-    // nothing for this CTA
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
   } else if (warp == 0) {
-    // ---- run list, K and V ----
-    const int64_t x0 = sp_first(cta, W, n_used), x1 = sp_first(cta + 1, W, n_used);
-    const int n_seg = p.hdr[0];
-    const int64_t n_units = static_cast<int64_t>(n_seg) * p.HKV;
-    int64_t unit = static_cast<int64_t>(p.start[2 * cta]) * p.HKV + p.start[2 * cta + 1];
-    // a tile whose V still has to be asked for
-    int v_pages[2] = {-1, -1}, v_head = 0, v_n = 0;
-    bool have_v = false;
-    auto slot_for = [&](uint32_t bytes, uint32_t& dst, uint32_t& bar) -> bool {
-      const uint32_t s = issued % NS, round = issued / NS;
-      if (round > 0 && !wait(empty(s), (round - 1) & 1, aborted)) return false;
-      dst = s_ring + s * kSlot;
-      bar = full(s);
-      if (elect()) mbar_expect_tx(bar, bytes);
-      ++issued;
-      return true;
-    };
-    auto load_v = [&]() -> bool {
-      uint32_t dst, bar;
-      if (!slot_for(v_n * 16384, dst, bar)) return false;
-      if (elect())
-        for (int i = 0; i < v_n; ++i)
-          for (int h = 0; h < 2; ++h)
-            tma_load(dst + h * 16384 + i * 8192, &map_v, v_head * 256 + h * 128, v_pages[i] * kPage, bar);
-      return true;
-    };
+    // ---- run list, q, K and V ----
+    // waits for the next slot to be free
+    auto take = [&](uint32_t n) -> bool { return n < NS || wait(empty(n % NS), (n / NS - 1) & 1, aborted); };
     bool ok = true;
-    for (int c = 0; ok; ++c) {
-      if (c >= 2 && !wait(runempty(c & 1), ((c >> 1) - 1) & 1, aborted)) break;
-      const int64_t u = unit + lane;
-      Run r{};
-      int n = 0;
-      bool past = u >= n_units;
-      if (!past) {
-        const int si = static_cast<int>(u / p.HKV), head = static_cast<int>(u % p.HKV);
-        const SpSegment s = p.seg[si];
-        const int64_t pos = static_cast<int64_t>(p.cum[si]) * p.HKV + static_cast<int64_t>(head) * sp_cost(s.tiles) + kSpUnitCost;
-        past = pos >= x1;
-        const int64_t a = pos > x0 ? pos : x0, b = pos + s.tiles < x1 ? pos + s.tiles : x1;
-        if (b > a) {
-          n = static_cast<int>(b - a);
-          r.table_row = s.table_row; r.row0 = s.row0; r.rows = s.rows; r.head = head;
-          r.tok0 = s.page0 * kPage + static_cast<int>(a - pos) * kSpTile;
-          r.end = s.end;
-          r.tiles = n;
-          r.small = s.rows <= 8;
-          r.part = sp_part_row(p, s, head, cta);
-        }
-      }
-      const uint32_t live = __ballot_sync(0xffffffffu, n > 0);
-      const int is_last = __any_sync(0xffffffffu, past) ? 1 : 0, n_runs = __popc(live);
-      if (n > 0) runs[(c & 1) * kRunChunk + __popc(live & ((1u << lane) - 1u))] = r;
-      if (lane == 0) { run_head[2 * (c & 1)] = n_runs; run_head[2 * (c & 1) + 1] = is_last; }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(runfull(c & 1));
-      unit += 32;
-      for (int j = 0; j < n_runs && ok; ++j) {
-        const Run q = runs[(c & 1) * kRunChunk + j];
-        const int32_t* row = p.bt + static_cast<int64_t>(q.table_row) * p.bt_stride;
-        const int col0 = q.tok0 / kPage, cols = (q.end + kPage - 1) / kPage;     // cols <= p.cols
-        auto page_at = [&](int col) {
-          const int x = col < cols ? row[col] : -1;
-          return x >= 0 && x < p.n_pages ? x : -1;     // TMA reads zeros at negative rows
-        };
-        int ids = page_at(col0 + lane), ids_next = page_at(col0 + 32 + lane);
-        for (int t = 0; t < q.tiles; ++t) {
-          if (t > 0 && (t & 15) == 0) { ids = ids_next; ids_next = page_at(col0 + 2 * t + 32 + lane); }
-          const int n_pages = min(2, cols - (col0 + 2 * t));
-          const int pg0 = __shfl_sync(0xffffffffu, ids, (2 * t) & 31), pg1 = __shfl_sync(0xffffffffu, ids, (2 * t + 1) & 31);
-          uint32_t dst, bar;
-          if (!slot_for(n_pages * (p.r ? 16384 : 8192), dst, bar)) { ok = false; break; }
-          if (elect())
-            for (int i = 0; i < n_pages; ++i) {
-              const int y = (i ? pg1 : pg0) * kPage;
-              tma_load(dst + i * 8192, &map_k, q.head * 128, y, bar);
-              if (p.r) tma_load(dst + kPiece + i * 8192, &map_r, q.head * 128, y, bar);
-            }
-          if (have_v && !load_v()) { ok = false; break; }
-          v_pages[0] = pg0; v_pages[1] = pg1; v_head = q.head; v_n = n_pages;
-          have_v = true;
-        }
-      }
-      if (is_last) break;
-    }
-    if (ok && have_v) load_v();
-  } else if (warp == 1) {
-    // ---- MMA ----
-    const uint32_t idesc_s = instr(0, p.fp8 == FFA_E4M3 ? 0 : 1, 0), idesc_o = instr(VBF16 ? 1 : 0, VBF16 ? 1 : 0, 1);
-    uint32_t used = 0;                        // slots consumed
-    uint32_t i = 0;                           // tiles whose QK was issued
-    int n_run = 0;
-    // the tile whose PV is still to come
-    bool have = false, first = false;
-    int valid = 0, o_buf = 0, o_round = 0;
-    auto pv = [&]() -> bool {
-      const uint32_t j = i - 1, s = used % NS;
-      if (!wait(full(s), (used / NS) & 1, aborted)) return false;
-      const uint32_t v = s_ring + s * kSlot;
-      const int steps = (valid + 15) / 16;
-      if (valid < steps * 16) {
-        // tokens past the end of the sequence: whatever their V holds, 0 * V has to be 0
-        for (int x = lane; x < (steps * 16 - valid) * 16; x += 32) {
-          const int row = valid + x / 16, h = (x >> 3) & 1, ck = x & 7;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(v + h * 16384 + row * 128 + ck * 16), "r"(0) : "memory");
-        }
-        fence_async();
-        __syncwarp();
-      }
-      if (first && o_round > 0 && !wait(ofree(o_buf), (o_round - 1) & 1, aborted)) return false;
-      if (!wait(pfull(j & 1), (j >> 1) & 1, aborted)) return false;
-      fence_after();
-      if (elect()) {
-        const uint64_t dv = desc(v, 16384);
-        for (int k = 0; k < steps; ++k)
-          mma_16_tmem(tmem + 256 + 128 * o_buf, tmem + 128 * (j & 1) + 8 * k, dv + 128 * k, idesc_o, !(first && k == 0));
-        commit(empty(s));
-        commit(odone);
+    uint32_t listed = 0;
+    auto list = [&](const Run& r) -> bool {
+      const uint32_t i = listed % kRuns, round = listed / kRuns;
+      if (round > 0 && !wait(runempty(i), (round - 1) & 1, aborted)) return false;
+      if (lane == 0) {
+        runs[i] = r;
+        mbar_arrive(runfull(i));
       }
       __syncwarp();
-      ++used;
+      ++listed;
       return true;
     };
+    uint32_t q_large = 0, q_small = 0;
+    auto load_q = [&](const Run& r) -> bool {
+      const bool small = r.small != 0;
+      const uint32_t qb = small ? 1 + (q_small & 1) : 0, round = small ? q_small >> 1 : q_large;
+      if (round > 0 && !wait(qfree(qb), (round - 1) & 1, aborted)) return false;
+      if (small) ++q_small; else ++q_large;
+      if (listed == 1) {                      // before the first q: the kernel that splits it has ended
+        asm volatile("griddepcontrol.wait;\n" ::: "memory");
+        asm volatile("fence.proxy.async.global;\n" ::: "memory");   // its pieces were written by ordinary stores
+      }
+      if (elect()) {
+        const int rows_head = p.B * p.G;
+        const uint32_t bytes = small ? 1024 : kPiece;
+        mbar_expect_tx(qfull(qb), NP * bytes);
+        for (int piece = 0; piece < NP; ++piece)
+          tma_load(q_buffer(qb) + piece * bytes, small ? &map_q8 : &map_q, 0, (piece * p.HKV + r.head) * rows_head + r.row0, qfull(qb));
+      }
+      __syncwarp();
+      return true;
+    };
+    // q of a later run is asked for after the run's first tile, which need not wait until a q buffer is free
+    auto load = [&](const Run& r) -> bool {
+      if (listed == 1 && !load_q(r)) return false;
+      const int32_t* row = p.bt + static_cast<int64_t>(r.table_row) * p.bt_stride;
+      const int col0 = r.tok0 / kPage, cols = (r.end + kPage - 1) / kPage;         // cols <= p.cols
+      auto page_at = [&](int col) {
+        const int y = col < cols ? row[col] : -1;
+        return y >= 0 && y < p.n_pages ? y : -1;       // TMA reads zeros at negative rows
+      };
+      int ids = page_at(col0 + lane), ids_next = page_at(col0 + 32 + lane);
+#pragma unroll 1
+      for (int t = 0; t < r.tiles; ++t) {
+        if (t > 0 && (t & 15) == 0) { ids = ids_next; ids_next = page_at(col0 + 2 * t + 32 + lane); }
+        const int n_pages = min(2, cols - (col0 + 2 * t));
+        const int y0 = __shfl_sync(0xffffffffu, ids, (2 * t) & 31) * kPage, y1 = __shfl_sync(0xffffffffu, ids, (2 * t + 1) & 31) * kPage;
+        // K base and K residual: a box of 64 tokens x 128 bytes for either page; V of either page: 64 tokens x 2 x 128 bytes
+        if (!take(issued) || (nk > 1 && !take(issued + 1))) return false;
+        const uint32_t s0 = issued % NS, s1 = (issued + 1) % NS;
+        if (elect()) {
+          const uint32_t d0 = s_ring + s0 * kSlot, d1 = s_ring + s1 * kSlot;
+          mbar_expect_tx(full(s0), n_pages * 8192);
+          tma_load(d0, &map_k, r.head * 128, y0, full(s0));
+          if (n_pages > 1) tma_load(d0 + 8192, &map_k, r.head * 128, y1, full(s0));
+          if (nk > 1) {
+            mbar_expect_tx(full(s1), n_pages * 8192);
+            tma_load(d1, &map_r, r.head * 128, y0, full(s1));
+            if (n_pages > 1) tma_load(d1 + 8192, &map_r, r.head * 128, y1, full(s1));
+          }
+        }
+        issued += nk;
+        if (!take(issued) || (n_pages > 1 && !take(issued + 1))) return false;
+        const uint32_t s2 = issued % NS, s3 = (issued + 1) % NS;
+        if (elect()) {
+          mbar_expect_tx(full(s2), 16384);
+          tma_load_3d(s_ring + s2 * kSlot, &map_v, 0, y0, 2 * r.head, full(s2));
+          if (n_pages > 1) {
+            mbar_expect_tx(full(s3), 16384);
+            tma_load_3d(s_ring + s3 * kSlot, &map_v, 0, y1, 2 * r.head, full(s3));
+          }
+        }
+        issued += n_pages;
+        if (t == 0 && listed > 1 && !load_q(r)) return false;
+      }
+      return true;
+    };
+    int place = s_plan[13];
+    // the runs of one item
+    auto runs_of = [&](const SpItem& it, bool own) -> bool {
+      const int unit = sp_unit_cost(it.tiles), before = x0 - place - kSpBegin - (it.tiles - 1) * kSpTileCost;
+      int k = before <= 0 ? 0 : (before - 1) / unit + 1;                          // units that end before x0 are other CTAs'
+      int block = k / p.HKV, head = k - block * p.HKV;
+#pragma unroll 1
+      for (; k < it.units; ++k) {
+        const int first = place + k * unit + kSpBegin;                            // where tile 0 stands
+        if (first >= x1) break;
+        const int t0 = first >= x0 ? 0 : (x0 - first - 1) / kSpTileCost + 1;
+        const int t1 = min(it.tiles, (x1 - first - 1) / kSpTileCost + 1);
+        Run r;
+        r.table_row = it.first;
+        r.head = head;
+        r.row0 = it.first * p.G + block * kSpRows;
+        r.rows = min(kSpRows, it.rows - block * kSpRows);
+        r.tok0 = it.page0 * kPage + t0 * kSpTile;
+        r.end = it.end;
+        r.tiles = t1 - t0;
+        r.small = r.rows <= 8;
+        r.part = sp_part_row(p, own, r.row0, r.rows, head, cta);
+        if (!list(r) || !load(r)) return false;
+        if (++head == p.HKV) { head = 0; ++block; }
+      }
+      place += it.units * unit;
+      return true;
+    };
+    const int first_item = s_plan[12];
+    SpItem it = *s_first;
+    ok = runs_of(it, first_item < p.B);
+#pragma unroll 1
+    for (int i0 = first_item + 1; ok && i0 < n_items && place < x1; i0 += 32) {
+      // 32 items, one to a lane; one that has tiles after the other
+      const int i = i0 + lane;
+      SpItem x{};
+      if (i < n_items) x = sp_item(p, bounds, i, i < p.B ? p.seq_lens[i] : 0);
+      uint32_t todo = __ballot_sync(0xffffffffu, x.tiles > 0 && x.units > 0);
+#pragma unroll 1
+      while (todo && ok && place < x1) {
+        const int from = __ffs(todo) - 1;
+        todo &= todo - 1;
+        it.first = __shfl_sync(0xffffffffu, x.first, from);
+        it.rows = __shfl_sync(0xffffffffu, x.rows, from);
+        it.page0 = __shfl_sync(0xffffffffu, x.page0, from);
+        it.end = __shfl_sync(0xffffffffu, x.end, from);
+        it.tiles = __shfl_sync(0xffffffffu, x.tiles, from);
+        it.units = __shfl_sync(0xffffffffu, x.units, from);
+        ok = runs_of(it, i0 + from < p.B);
+      }
+    }
+    if (ok) {
+      Run none{};
+      list(none);
+    }
+  } else if (warp == 1) {
+    // ---- S = q K^T ----
+    const uint32_t idesc = instr(0, p.fp8 == FFA_E4M3 ? 0 : 1, 0);
+    uint32_t pos = 0, e = 0;                  // slots of the tiles before the present one, steps before it
+    uint32_t q_large = 0, q_small = 0;        // runs with the large or a small q buffer
     Run r;
     bool ok = true;
-    uint32_t q_large = 0, q_small = 0;        // runs of either kind so far
     while (ok && next_run(r)) {
       const uint32_t qb = r.small ? 1 + (q_small & 1) : 0;
       if (!wait(qfull(qb), (r.small ? q_small >> 1 : q_large) & 1, aborted)) break;
       if (r.small) ++q_small; else ++q_large;
-      fence_after();
       const uint64_t dq = desc(q_buffer(qb), 16);
-      const uint32_t q_step = q_piece[r.small ? 1 : 0] >> 4;
-      for (int t = 0; t < r.tiles; ++t) {
-        const uint32_t s = used % NS;
-        if (!wait(full(s), (used / NS) & 1, aborted)) { ok = false; break; }
+      const uint32_t q_step = (r.small ? 1024 : kPiece) >> 4;
+      for (int t = 0; t < r.tiles; ++t, ++e) {
+        const uint32_t s0 = pos % NS, s1 = (pos + 1) % NS, g = e & 1;
+        if (!wait(full(s0), (pos / NS) & 1, aborted)) { ok = false; break; }
+        if (nk > 1 && !wait(full(s1), ((pos + 1) / NS) & 1, aborted)) { ok = false; break; }
+        if (e >= 2 && !wait(sfree(g), ((e >> 1) - 1) & 1, aborted)) { ok = false; break; }
         fence_after();
         if (elect()) {
-          const uint64_t dk = desc(s_ring + s * kSlot, 16);
-          uint32_t acc = 0;
-          for (int part = 0; part < (p.r ? 2 : 1); ++part)
+          const uint64_t dk0 = desc(s_ring + s0 * kSlot, 16), dk1 = desc(s_ring + s1 * kSlot, 16);
+          const uint32_t d = tmem + 128 * g;
+#pragma unroll
+          for (int piece = 0; piece < NP; ++piece)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_fp8(d, dq + piece * q_step + 2 * k, dk0 + 2 * k, idesc, piece + k > 0);
+          if (nk > 1) {
 #pragma unroll
             for (int piece = 0; piece < NP; ++piece)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                mma_fp8(tmem + 128 * (i & 1), dq + piece * q_step + 2 * k, dk + (part * kPiece >> 4) + 2 * k, idesc_s, acc);
-                acc = 1;
-              }
-          commit(empty(s));
-          commit(sfull(i & 1));
+              for (int k = 0; k < 4; ++k) mma_fp8(d, dq + piece * q_step + 2 * k, dk1 + 2 * k, idesc, 1);
+          }
+          commit(sfull(g));
+          commit(empty(s0));
+          if (nk > 1) commit(empty(s1));
           if (t == r.tiles - 1) commit(qfree(qb));
         }
         __syncwarp();
-        ++used;
-        if (have && !pv()) { ok = false; break; }
-        ++i;
-        have = true;
-        first = t == 0;
-        valid = min(kSpTile, r.end - (r.tok0 + t * kSpTile));
-        o_buf = n_run & 1;
-        o_round = n_run >> 1;
+        pos += nk + (r.end - (r.tok0 + t * kSpTile) > kPage ? 2 : 1);
       }
-      ++n_run;
     }
-    if (ok && have && *reinterpret_cast<volatile int*>(aborted) == 0) pv();
   } else if (warp == 2) {
-    // ---- q ----
-    uint32_t q_large = 0, q_small = 0;
-    const int rows_head = p.B * p.G;
+    // ---- O += P V ----
+    const uint32_t idesc = instr(VBF16 ? 1 : 0, VBF16 ? 1 : 0, 1);
+    uint32_t pos = 0, e = 0, n_run = 0;
     Run r;
-    asm volatile("fence.proxy.async.global;\n" ::: "memory");       // q's pieces were written by ordinary stores
-    while (next_run(r)) {
-      const uint32_t qb = r.small ? 1 + (q_small & 1) : 0, round = r.small ? q_small >> 1 : q_large;
-      if (round > 0 && !wait(qfree(qb), (round - 1) & 1, aborted)) break;
-      if (r.small) ++q_small; else ++q_large;
-      if (elect()) {
-        const uint32_t bytes = q_piece[r.small ? 1 : 0];
-        mbar_expect_tx(qfull(qb), NP * bytes);
-        for (int piece = 0; piece < NP; ++piece)
-          tma_load(q_buffer(qb) + piece * bytes, r.small ? &map_q8 : &map_q, 0, (piece * p.HKV + r.head) * rows_head + r.row0, qfull(qb));
+    bool ok = true;
+    while (ok && next_run(r)) {
+      const uint32_t o = n_run & 1, d = tmem + 256 + 128 * o;
+      if (n_run >= 2 && !wait(ofree(o), ((n_run >> 1) - 1) & 1, aborted)) break;
+      ++n_run;
+      for (int t = 0; t < r.tiles && ok; ++t, ++e) {
+        const int valid = min(kSpTile, r.end - (r.tok0 + t * kSpTile)), pages = valid > kPage ? 2 : 1;
+        const uint32_t g = e & 1;
+        pos += nk;
+        for (int i = 0; i < pages && ok; ++i) {
+          const uint32_t n = pos + i, v = s_ring + n % NS * kSlot;
+          if (!wait(full(n % NS), (n / NS) & 1, aborted)) { ok = false; break; }
+          const int here = valid - i * kPage;
+          if (here < kPage && here % 16) {
+            // tokens past the end of the sequence: whatever their V holds, 0 * V has to be 0
+            for (int x = lane; x < (16 - here % 16) * 16; x += 32) {
+              const int row = here + x / 16, h = (x >> 3) & 1, ck = x & 7;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(v + h * 8192 + row * 128 + ck * 16), "r"(0) : "memory");
+            }
+            fence_async();
+            __syncwarp();
+          }
+        }
+        if (!ok || !wait(pfull(g), (e >> 1) & 1, aborted)) { ok = false; break; }
+        fence_after();
+        if (elect()) {
+          const uint32_t a = tmem + 128 * g;
+          for (int i = 0; i < pages; ++i) {
+            const uint64_t dv = desc(s_ring + (pos + i) % NS * kSlot, 8192);
+            const int ks = min(4, (valid - i * kPage + 15) / 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (k < ks) mma_16_tmem(d, a + 32 * i + 8 * k, dv + 128 * k, idesc, t > 0 || i + k > 0);
+          }
+          commit(sfree(g));
+          for (int i = 0; i < pages; ++i) commit(empty((pos + i) % NS));
+        }
+        __syncwarp();
+        pos += pages;
       }
-      __syncwarp();
     }
   } else if (warp >= 4) {
     // ---- softmax: one query row per thread ----
     const int quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    uint32_t i = 0;
-    int n_run = 0;
-    bool have_o = false, o_live = false;      // a finished run whose O is still to be written
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint32_t e = 0, n_run = 0;
+    // a finished run whose O is still to be written
+    bool have_o = false, o_live = false;
     int64_t o_part = 0;
+    int o_rows = 0;
     float o_m = 0.f, o_l = 0.f;
-    auto write_o = [&](int buf) {
+    auto write_o = [&](uint32_t o) {
       if (__any_sync(0xffffffffu, o_live)) {
-        float4* dst = reinterpret_cast<float4*>(p.part_o + (o_part + row) * kHeadDim);
-#pragma unroll
+        float4* const dst = p.part_o + 32 * o_part + row;
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t x[32];
-          tmem_ld32(x, tmem + lanes + 256 + 128 * buf + 32 * c);
+          tmem_ld32(x, lanes + 256 + 128 * o + 32 * c);
           tmem_wait_ld();
           if (o_live)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[8 * c + e] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]), __uint_as_float(x[4 * e + 2]),
-                                           __uint_as_float(x[4 * e + 3]));
+            for (int i = 0; i < 8; ++i)
+              dst[static_cast<int64_t>(8 * c + i) * o_rows] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]),
+                                                                          __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3]));
         }
         if (o_live) p.part_ml[o_part + row] = make_float2(o_m, o_l);
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ofree(buf));
+      if (lane == 0) mbar_arrive(ofree(o));
     };
     Run r;
     bool ok = true;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     while (ok && next_run(r)) {
       const bool live = row < r.rows, any_live = quarter * 32 < r.rows;
       float m = -INFINITY, l = 0.f, scale = 0.f;
@@ -485,77 +649,122 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
         scale = p.q_scale[static_cast<int64_t>(r.head) * p.B * p.G + r.row0 + row];
         end = min(end, p.seq_lens[(r.row0 + row) / p.G]);
       }
-      for (int t = 0; t < r.tiles; ++t, ++i) {
-        const uint32_t s_addr = tmem + lanes + 128 * (i & 1);
-        if (!wait(sfull(i & 1), (i >> 1) & 1, aborted)) { ok = false; break; }
+      const uint32_t o_addr = lanes + 256 + 128 * (n_run & 1);
+      for (int t = 0; t < r.tiles; ++t, ++e) {
+        const uint32_t g = e & 1, s_addr = lanes + 128 * g;
+        if (!wait(sfull(g), (e >> 1) & 1, aborted)) { ok = false; break; }
         fence_after();
-        uint32_t x[128];
-        float up = 1.f;                       // factor of what was summed so far
-        bool lift = false;
+        // PV of the step before is done: O may be brought down, and P of that step is not needed any more
+        bool waited = false;
+        auto pv_done = [&]() -> bool {
+          if (e > 0 && !waited && !wait(sfree(g ^ 1), ((e - 1) >> 1) & 1, aborted)) return false;
+          waited = true;
+          fence_after();
+          return true;
+        };
         if (any_live) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_addr + 32 * c);
-          tmem_wait_ld();
           const int lim = end - (r.tok0 + t * kSpTile);
-          if (__any_sync(0xffffffffu, lim < kSpTile)) {
+          const bool cut = __any_sync(0xffffffffu, lim < kSpTile);
+          uint32_t x[128];
+          float top = -INFINITY;
+          if (!cut) {
 #pragma unroll
-            for (int e = 0; e < 128; ++e) x[e] = e < lim ? x[e] : 0xff800000u;
-          }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_addr + 32 * c);
+            tmem_wait_ld();
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 128; ++e) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(x[e]));
-          const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-          // the reference point moves only when a weight would pass 2^8: rarely, and O is rescaled only then
-          if (tile_top > m + 8.f || m == -INFINITY) {
-            const float to = fmaxf(m, tile_top);
-            up = m == -INFINITY ? 0.f : ex2(m - to);
-            lift = t > 0 && to > m;
-            m = to;
-          }
-          const float neg = m == -INFINITY ? 0.f : -m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 128; i += 8)
 #pragma unroll
-          for (int e = 0; e < 128; e += 2) {
-            const float a = ex2(fmaf(__uint_as_float(x[e]), scale, neg)), b = ex2(fmaf(__uint_as_float(x[e + 1]), scale, neg));
-            sum[(e >> 1) & 3] += a + b;
-            x[e >> 1] = pack16<VBF16>(a, b);
-          }
-          l = l * up + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-        }
-        // PV of the tile before has read its P and finished with O
-        if (i > 0 && !wait(odone, (i - 1) & 1, aborted)) { ok = false; break; }
-        fence_after();
-        if (any_live) {
-          if (__any_sync(0xffffffffu, lift)) {
+              for (int j = 0; j < 4; ++j) tops[j] = max3(tops[j], __uint_as_float(x[i + j]), __uint_as_float(x[i + j + 4]));
+            top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+          } else {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
               uint32_t y[32];
-              const uint32_t o_addr = tmem + lanes + 256 + 128 * (n_run & 1) + 32 * c;
-              tmem_ld32(y, o_addr);
+              tmem_ld32(y, s_addr + 32 * c);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * up);
-              tmem_st32(o_addr, y);
+              for (int i = 0; i < 32; ++i)
+                if (32 * c + i < lim) top = max3(top, __uint_as_float(y[i]), __uint_as_float(y[i]));
             }
           }
-          tmem_st32(s_addr, x);
-          tmem_st32(s_addr + 32, x + 32);
+          top = live ? top * scale : 0.f;     // the other lanes' S is whatever lay in shared memory
+          // the reference point moves only when a weight would pass 2^8: rarely, and O is rescaled only then
+          float up = 1.f;
+          bool lift = false;
+          if (!(top <= m + 8.f) || m == -INFINITY) {
+            const float to = top > m || top != top ? top : m;      // NaN stays and makes the row NaN
+            up = m == -INFINITY ? 0.f : ex2(m - to);
+            lift = t > 0 && !(to <= m);
+            m = to;
+          }
+          if (__any_sync(0xffffffffu, lift)) {
+            if (!pv_done()) { ok = false; break; }
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t y[16];
+              tmem_ld16(y, o_addr + 16 * c);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * up);
+              tmem_st16(o_addr + 16 * c, y);
+            }
+          }
+          const float neg = m == -INFINITY ? 0.f : -m;
+          float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+          if (!cut) {
+#pragma unroll
+            for (int i = 0; i < 128; i += 4) {
+              float2 a = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale, neg);
+              float2 b = fma2(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale, neg);
+              a = make_float2(ex2(a.x), ex2(a.y));
+              b = make_float2(ex2(b.x), ex2(b.y));
+              sum = add2(sum, a);
+              sum1 = add2(sum1, b);
+              x[i / 2] = pack16<VBF16>(a.x, a.y);
+              x[i / 2 + 1] = pack16<VBF16>(b.x, b.y);
+            }
+            tmem_st32(s_addr, x);
+            tmem_st32(s_addr + 32, x + 32);
+          } else {
+            // P of 32 tokens takes 16 columns, so it never reaches an S that is still to be read
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t y[32];
+              tmem_ld32(y, s_addr + 32 * c);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float2 a = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), scale, neg);
+                a = make_float2(32 * c + i < lim ? ex2(a.x) : 0.f, 32 * c + i + 1 < lim ? ex2(a.y) : 0.f);
+                sum = add2(sum, a);
+                y[i / 2] = pack16<VBF16>(a.x, a.y);
+              }
+              tmem_st16(s_addr + 16 * c, y);
+            }
+          }
+          l = l * up + ((sum.x + sum.y) + (sum1.x + sum1.y));
           tmem_wait_st();
         }
+        if (!pv_done()) { ok = false; break; }
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pfull(i & 1));
-        if (t == 0 && have_o) { write_o((n_run - 1) & 1); have_o = false; }
+        if (lane == 0) mbar_arrive(pfull(g));
+        if (t == 0 && have_o) {
+          write_o((n_run - 1) & 1);
+          have_o = false;
+        }
       }
       if (!ok) break;
       have_o = true;
       o_live = live;
       o_part = r.part;
+      o_rows = r.rows;
       o_m = m;
       o_l = l;
       ++n_run;
     }
-    if (ok && have_o && wait(odone, (i - 1) & 1, aborted)) {
+    if (ok && have_o && wait(sfree((e - 1) & 1), ((e - 1) >> 1) & 1, aborted)) {
       fence_after();
       write_o((n_run - 1) & 1);
     }
@@ -566,14 +775,16 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   if (*aborted) {
     // what is still on its way must land before the CTA's memory is given up
     if (warp == 0) {
-      for (uint32_t n = issued > NS ? issued - NS : 0; n < issued; ++n) {
-        wait_lane(full(n % NS), (n / NS) & 1, aborted + 1);
-      }
-      if (lane == 0) { p.hdr[2] = 1; atomicExch(p.status, 1); }
+      for (uint32_t n = issued > NS ? issued - NS : 0; n < issued; ++n) wait_lane(full(n % NS), (n / NS) & 1, aborted + 1);
+      if (lane == 0) { p.hdr[1] = 1; atomicExch(p.status, 1); }
     } else if (warp == 1) {
-      if (lane == 0) commit(final_bar);
+      if (elect()) commit(final_bar(0));
       __syncwarp();
-      wait_lane(final_bar, 0, aborted + 1);
+      wait_lane(final_bar(0), 0, aborted + 1);
+    } else if (warp == 2) {
+      if (elect()) commit(final_bar(1));
+      __syncwarp();
+      wait_lane(final_bar(1), 0, aborted + 1);
     }
     __syncthreads();
   }
@@ -599,12 +810,15 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// Rows of `row_bytes`; a box is 128 bytes of box_rows of them, 128-byte swizzle.
-bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t row_bytes, uint32_t box_rows, CUtensorMapL2promotion promo) {
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
-  const cuuint32_t box[2] = {128, box_rows}, ones[2] = {1, 1};
-  return encode_tiled()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones,
+// Rows of `row_bytes`; a box is 128 bytes of box_rows of them, 128-byte swizzle.  With `chunks` the box has that many
+// 128-byte pieces of every row, piece by piece.
+bool make_map(CUtensorMap* m, const void* base, int64_t rows, int64_t row_bytes, uint32_t box_rows, CUtensorMapL2promotion promo,
+              uint32_t chunks = 0) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(chunks ? 128 : row_bytes), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(row_bytes / 128)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes), 128};
+  const cuuint32_t box[3] = {128, box_rows, chunks}, ones[3] = {1, 1, 1};
+  return encode_tiled()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, chunks ? 3 : 2, const_cast<void*>(base), dims, strides, box, ones,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promo,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -644,8 +858,8 @@ int launch_sp_attend(const SpParams& p, cudaStream_t st) {
   // L2 promotion no wider than one head's row: the neighbouring heads belong to other units
   if (!make_map(&maps[0], p.k, rows, k_bytes, kPage, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
       !make_map(&maps[1], p.r ? p.r : p.k, rows, k_bytes, kPage, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
-      !make_map(&maps[2], p.v, rows, 2 * k_bytes, kPage, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
-      !make_map(&maps[3], p.qp, q_rows, 128, kSpRows, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+      !make_map(&maps[2], p.v, rows, 2 * k_bytes, kPage, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, 2) ||
+      !make_map(&maps[3], p.qp, q_rows, 128, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
       !make_map(&maps[4], p.qp, q_rows, 128, 8, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
     return FFA_E_LAUNCH;
   const bool two = p.q_dtype == FFA_BF16, bf = p.v_dtype == FFA_BF16;

@@ -324,7 +324,7 @@ int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* pools, int3
  * Sequence b of group g (group_start[g] <= b < group_start[g + 1]) has seq_lens[b] tokens; tokens below
  * 64 * prefix_pages[g] are in the pages that the table row of the group's FIRST sequence names, the others in those of
  * its own row.  A sequence shorter than the prefix sees its first seq_lens[b] tokens; one of length 0 gives zeros.  A
- * sequence outside every group has no shared part.  All of this is device memory and is read by the kernels, so a
+ * sequence outside every group has no shared part, nor has any if the bounds do not ascend.  All of this is device memory and is read by the kernels, so a
  * captured call follows it.  Entries outside 0 .. n_pages - 1 read as zero keys and values.  The reference has no
  * counterpart (its sequences share nothing).
  */
