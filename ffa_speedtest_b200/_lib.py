@@ -195,8 +195,11 @@ def current_stream(device) -> int:
 
 def enqueue(device: torch.device, fn, what: str, *args) -> None:
     """Call ``fn(*args, stream)`` on ``device`` and its current stream, whichever device is the current one."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)

@@ -24,6 +24,13 @@ enum { kHdrOk = 0, kHdrJobs = 1, kHdrLive = 2, kHdrArrive = 3, kHdrInts = 16 };
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPage - 1) / kPage; }
 
+// Every kernel here is launched while the one before it in the stream may still run (programmatic dependent launch): it
+// is set up meanwhile and waits for that one's end before it reads anything.
+__device__ __forceinline__ void begin() {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+
 struct Table {
   int n_pages, max_seqs, cols, stride;
   int32_t* block_table;
@@ -94,6 +101,7 @@ __device__ __forceinline__ bool check_seqs(const int32_t* seqs, int n, int max_s
 __global__ void __launch_bounds__(128) truncate_kernel(Table t, const int32_t* __restrict__ seqs,
                                                        const int32_t* __restrict__ new_lens, int n) {
   __shared__ int s_old;
+  begin();
   bool bad = false;
   for (int i = threadIdx.x; i < n; i += blockDim.x) bad |= seqs[i] < 0 || seqs[i] >= t.max_seqs || new_lens[i] < 0;
   if (__syncthreads_or(bad)) {
@@ -119,6 +127,7 @@ __global__ void __launch_bounds__(256) fork_kernel(Table t, const int32_t* __res
                                                    const int32_t* __restrict__ children, int n) {
   extern __shared__ uint32_t s_bits[];
   __shared__ int s_last;
+  begin();
   bool ok = check_seqs(children, n, t.max_seqs, true, s_bits);
   if (ok) {
     bool bad = false;
@@ -158,7 +167,14 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, cons
   extern __shared__ uint32_t s_bits[];
   __shared__ int s_warp[33];
   __shared__ int s_count[kPlanThreads / 32];
+  begin();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // free pages: every warp counts its stretch of the reference counts (and lists them from its place on, below)
+  const int per = (((t.n_pages + 31) / 32 + 31) / 32) * 32;          // a stretch in whole rows of 32
+  const int from = min(t.n_pages, warp * per), to = min(t.n_pages, from + per);
+  int n_free = 0;
+#pragma unroll 4
+  for (int p = from + lane; p < to; p += 32) n_free += t.refcount[p] == 0;
   bool ok = check_seqs(seqs, n, t.max_seqs, true, s_bits);
   if (ok) {
     bool bad = false;
@@ -195,16 +211,10 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, cons
     if (i < n) t.first_new()[i] = total + before;
     total += sum;
   }
-  // free pages: every warp counts its stretch of the reference counts, then lists it from its place on
   int found = 0;
   if (total > 0) {
-    const int per = (((t.n_pages + 31) / 32 + 31) / 32) * 32;        // a stretch in whole rows of 32
-    const int from = min(t.n_pages, warp * per), to = min(t.n_pages, from + per);
-    int mine = 0;
-    for (int p = from + lane; p < to; p += 32) mine += t.refcount[p] == 0;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-    if (lane == 0) s_count[warp] = mine;
+    n_free = __reduce_add_sync(0xffffffffu, n_free);
+    if (lane == 0) s_count[warp] = n_free;
     __syncthreads();
     int at = 0;
     for (int w = 0; w < 32; ++w) {
@@ -226,30 +236,43 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, cons
     if (tid == 0) { atomicOr(t.status, FFA_PAGES_NO_SPACE); hdr[kHdrJobs] = 0; }
     return;
   }
-  for (int i = warp; i < n; i += kPlanThreads / 32) {
-    const int add = n_new[i];
-    if (add == 0) continue;
-    const int s = seqs[i], len = t.seq_lens[s];
-    int32_t* row = t.row(s);
-    int first = t.first_new()[i];
-    if (t.job_src()[i] >= 0) {
-      if (lane == 0) {
-        const int p = t.free_list()[first];
+  // a thread to a sequence; one that needs many pages leaves them to its warp
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int c0 = 0, c1 = 0, first = 0, s = 0;
+    if (i < n && n_new[i] > 0) {
+      s = seqs[i];
+      const int len = t.seq_lens[s], add = n_new[i];
+      int32_t* row = t.row(s);
+      first = t.first_new()[i];
+      if (t.job_src()[i] >= 0) {
+        const int p = t.free_list()[first++];
         atomicSub(t.refcount + t.job_src()[i], 1);
         t.job_dst()[i] = p;
         row[len / kPage] = p;
         t.refcount[p] = 1;
       }
-      ++first;
+      c0 = pages_of(len);
+      c1 = pages_of(len + add);
+      if (c1 - c0 <= 4) {
+        for (; c0 < c1; ++c0, ++first) {
+          const int p = t.free_list()[first];
+          row[c0] = p;
+          t.refcount[p] = 1;
+        }
+      }
+      t.seq_lens[s] = len + add;
     }
-    const int c0 = pages_of(len), c1 = pages_of(len + add);
-    for (int c = c0 + lane; c < c1; c += 32) {
-      const int p = t.free_list()[first + c - c0];
-      row[c] = p;
-      t.refcount[p] = 1;
+    for (uint32_t todo = __ballot_sync(0xffffffffu, c0 < c1); todo; todo &= todo - 1) {
+      const int from = __ffs(todo) - 1;
+      const int a = __shfl_sync(0xffffffffu, c0, from), b = __shfl_sync(0xffffffffu, c1, from), f = __shfl_sync(0xffffffffu, first, from);
+      int32_t* row = t.row(__shfl_sync(0xffffffffu, s, from));
+      for (int c = a + lane; c < b; c += 32) {
+        const int p = t.free_list()[f + c - a];
+        row[c] = p;
+        t.refcount[p] = 1;
+      }
     }
-    __syncwarp();
-    if (lane == 0) t.seq_lens[s] = len + add;
   }
   if (tid == 0) hdr[kHdrJobs] = n;
 }
@@ -260,6 +283,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, cons
 // number.  job_rows(): the reference counts of the moved pages.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(Table t) {
   __shared__ int s_live[32], s_hole[32], s_move[32];
+  begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (((t.n_pages + 31) / 32 + 31) / 32) * 32;
   const int from = min(t.n_pages, warp * per), to = min(t.n_pages, from + per);
@@ -312,16 +336,16 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(Table t) {
 
 // Rewrites block table and reference counts entry by entry; out may be the state itself.  Only pages numbered
 // `live` or above are renamed, and the reference count of every entry below depends on that entry alone.
-__global__ void __launch_bounds__(256) compact_apply_kernel(Table t, int32_t* bt_out, int32_t* rc_out) {
-  const int live = t.hdr()[kHdrLive];
-  const int64_t n_entries = static_cast<int64_t>(t.max_seqs) * t.cols, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  for (int64_t i = i0; i < n_entries; i += step) {
-    const int64_t at = i / t.cols * t.stride + i % t.cols;
-    const int p = t.block_table[at];
-    bt_out[at] = p >= live && p < t.n_pages ? t.free_list()[p] : p;
+__device__ __forceinline__ void compact_apply(const Table& t, int32_t* bt_out, int32_t* rc_out, int block, int blocks) {
+  const int live = t.hdr()[kHdrLive], warps = blocks * kCopyThreads / 32, lane = threadIdx.x & 31;
+  for (int s = (block * kCopyThreads + threadIdx.x) / 32; s < t.max_seqs; s += warps) {
+    const int64_t at = static_cast<int64_t>(s) * t.stride;
+    for (int j = lane; j < t.cols; j += 32) {
+      const int p = t.block_table[at + j];
+      bt_out[at + j] = p >= live && p < t.n_pages ? t.free_list()[p] : p;
+    }
   }
-  for (int64_t i = i0; i < t.n_pages; i += step) {
+  for (int i = block * kCopyThreads + threadIdx.x; i < t.n_pages; i += blocks * kCopyThreads) {
     const int c = t.refcount[i];
     rc_out[i] = i >= live ? 0 : c ? c : t.job_rows()[t.free_list()[i]];
   }
@@ -329,17 +353,22 @@ __global__ void __launch_bounds__(256) compact_apply_kernel(Table t, int32_t* bt
 
 // ---- page contents --------------------------------------------------------------------------------------
 // Copies the first rows(i) tokens of page src(i) to page dst(i) in every pool, all jobs of the header.  A block takes
-// 16 KiB pieces, piece number fastest, so that neighbouring blocks read and write one page together.
+// 16 KiB pieces, piece number fastest, so that neighbouring blocks read and write one page together.  COMPACT: whole pages,
+// and the first blocks rewrite table and counts before they join in.
+constexpr int kApplyBlocks = 64;
+template <bool COMPACT>
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(Table t, const uint64_t* __restrict__ bases,
                                                                   const int32_t* __restrict__ token_bytes, int n_pools,
-                                                                  int pieces, bool whole) {
+                                                                  int pieces, int32_t* bt_out, int32_t* rc_out) {
+  begin();
+  if (COMPACT && blockIdx.x < kApplyBlocks) compact_apply(t, bt_out, rc_out, blockIdx.x, min(kApplyBlocks, static_cast<int>(gridDim.x)));
   const int jobs = t.hdr()[kHdrJobs];
   const int64_t n_items = static_cast<int64_t>(jobs) * n_pools * pieces;
   for (int64_t item = blockIdx.x; item < n_items; item += gridDim.x) {
     const int piece = static_cast<int>(item % pieces);
     const int pool = static_cast<int>(item / pieces % n_pools);
     const int64_t job = item / pieces / n_pools;
-    const int rows = whole ? kPage : t.job_rows()[job];
+    const int rows = COMPACT ? kPage : t.job_rows()[job];
     const int64_t bytes = static_cast<int64_t>(rows) * token_bytes[pool], page = static_cast<int64_t>(kPage) * token_bytes[pool];
     const int64_t at = static_cast<int64_t>(piece) * kChunk;
     if (at >= bytes) continue;
@@ -359,11 +388,6 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(Table t, const
   }
 }
 
-int last_launch(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? FFA_OK : note_cuda_error(e, what);
-}
-
 int make_table(const FfaPageTable* a, Table* t) {
   if (!a || !a->block_table || !a->seq_lens || !a->refcount || !a->status || !a->scratch) return FFA_E_NULL;
   if (a->n_pages <= 0 || a->max_seqs <= 0 || a->cols <= 0 || a->bt_stride < a->cols || a->cols > INT32_MAX / kPage) return FFA_E_SHAPE;
@@ -374,13 +398,30 @@ int make_table(const FfaPageTable* a, Table* t) {
   return FFA_OK;
 }
 
-int launch_copy(const Table& t, const FfaPagePools* pools, int64_t max_jobs, bool whole, cudaStream_t st) {
-  if (pools->n_pools == 0 || max_jobs == 0) return FFA_OK;
+template <typename... P, typename... A>
+int launch(const char* what, void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? FFA_OK : note_cuda_error(e, what);
+}
+
+template <bool COMPACT>
+int launch_copy(const Table& t, const FfaPagePools* pools, int64_t max_jobs, int32_t* bt_out, int32_t* rc_out, cudaStream_t st) {
+  if (!COMPACT && pools->n_pools == 0) return FFA_OK;
   const int pieces = static_cast<int>((static_cast<int64_t>(kPage) * pools->max_token_bytes + kChunk - 1) / kChunk);
-  const int64_t items = max_jobs * pools->n_pools * pieces;
-  const unsigned blocks = static_cast<unsigned>(items < 148 * 8 ? items : 148 * 8);
-  copy_pages_kernel<<<blocks, kCopyThreads, 0, st>>>(t, pools->bases, pools->token_bytes, pools->n_pools, pieces, whole);
-  return last_launch("ffa_pages (copy)");
+  const int64_t items = max_jobs * pools->n_pools * pieces, least = COMPACT ? kApplyBlocks : 1;
+  const unsigned blocks = static_cast<unsigned>(items > 148 * 8 ? 148 * 8 : items > least ? items : least);
+  return launch("ffa_pages (copy)", copy_pages_kernel<COMPACT>, blocks, kCopyThreads, 0, st, t, pools->bases, pools->token_bytes,
+                pools->n_pools, pieces, bt_out, rc_out);
 }
 
 int check_pools(const FfaPagePools* p) {
@@ -408,8 +449,7 @@ extern "C" int ffa_pages_truncate(const FfaPageTable* table, const int32_t* seqs
   if (rc) return rc;
   if (!seqs || !new_lens) return FFA_E_NULL;
   if (n <= 0 || n > t.max_seqs) return FFA_E_SHAPE;
-  truncate_kernel<<<n, 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(t, seqs, new_lens, n);
-  return last_launch("ffa_pages_truncate");
+  return launch("ffa_pages_truncate", truncate_kernel, n, 128, 0, reinterpret_cast<cudaStream_t>(stream), t, seqs, new_lens, n);
 }
 
 extern "C" int ffa_pages_fork(const FfaPageTable* table, const int32_t* parents, const int32_t* children, int32_t n,
@@ -419,8 +459,7 @@ extern "C" int ffa_pages_fork(const FfaPageTable* table, const int32_t* parents,
   if (rc) return rc;
   if (!parents || !children) return FFA_E_NULL;
   if (n <= 0 || n > t.max_seqs) return FFA_E_SHAPE;
-  fork_kernel<<<n, 256, bits_bytes(t.max_seqs), reinterpret_cast<cudaStream_t>(stream)>>>(t, parents, children, n);
-  return last_launch("ffa_pages_fork");
+  return launch("ffa_pages_fork", fork_kernel, n, 256, bits_bytes(t.max_seqs), reinterpret_cast<cudaStream_t>(stream), t, parents, children, n);
 }
 
 extern "C" int ffa_pages_extend(const FfaPageTable* table, const FfaPagePools* pools, const int32_t* seqs,
@@ -432,9 +471,8 @@ extern "C" int ffa_pages_extend(const FfaPageTable* table, const FfaPagePools* p
   if (!seqs || !n_new) return FFA_E_NULL;
   if (n <= 0 || n > t.max_seqs) return FFA_E_SHAPE;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  extend_plan_kernel<<<1, kPlanThreads, bits_bytes(t.max_seqs), st>>>(t, seqs, n_new, n);
-  if ((rc = last_launch("ffa_pages_extend"))) return rc;
-  return launch_copy(t, pools, n, false, st);
+  if ((rc = launch("ffa_pages_extend", extend_plan_kernel, 1, kPlanThreads, bits_bytes(t.max_seqs), st, t, seqs, n_new, n))) return rc;
+  return launch_copy<false>(t, pools, n, nullptr, nullptr, st);
 }
 
 extern "C" int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* pools, int32_t* block_table_out,
@@ -445,11 +483,6 @@ extern "C" int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* 
   if ((rc = check_pools(pools))) return rc;
   if (!block_table_out || !refcount_out) return FFA_E_NULL;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(t);
-  if ((rc = last_launch("ffa_pages_compact"))) return rc;
-  const int64_t n = static_cast<int64_t>(t.max_seqs) * t.cols;
-  const int64_t blocks = ((n > t.n_pages ? n : t.n_pages) + 255) / 256;
-  compact_apply_kernel<<<static_cast<unsigned>(blocks < 148 * 4 ? blocks : 148 * 4), 256, 0, st>>>(t, block_table_out, refcount_out);
-  if ((rc = last_launch("ffa_pages_compact"))) return rc;
-  return launch_copy(t, pools, t.n_pages / 2, true, st);
+  if ((rc = launch("ffa_pages_compact", compact_plan_kernel, 1, kPlanThreads, 0, st, t))) return rc;
+  return launch_copy<true>(t, pools, t.n_pages / 2, block_table_out, refcount_out, st);
 }

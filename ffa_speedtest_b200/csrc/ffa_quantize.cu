@@ -45,24 +45,27 @@ struct RowMap {
 // writes whole 128-byte lines.  DT and F8 are compile-time so the per-element code has no branches
 // on the element type.
 template <int DT>
+__device__ __forceinline__ void unpack8(uint4 v, float (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (DT == kBF16) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <int DT>
 __device__ __forceinline__ void load8(const void* __restrict__ k, int64_t e, float (&x)[8]) {
   if (DT == kF32) {
     const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(k) + e);
     const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(k) + e + 4);
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(k) + e);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (DT == kBF16) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x; x[2 * i + 1] = f.y;
-      }
-    }
+    unpack8<DT>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(k) + e), x);
   }
 }
 
@@ -368,45 +371,48 @@ __global__ void __launch_bounds__(256) nvfp4_kernel(const void* __restrict__ k, 
   }
 }
 
-// K and V of new tokens to each sequence's own position.  A thread takes eight channels of one token: quantises K,
-// copies V.  Four tokens' loads are in flight per thread.  Tokens past counts[b], and positions without a page, are
-// left out: nothing is written for them.
+// K and V of new tokens to each sequence's own position.  A block takes kAppendRows tokens of one sequence, a thread
+// eight channels of a token at a time: quantises K, copies V; the loads of four are in flight per thread.  Bound by HBM
+// (512 bytes read and 512 written per token and kv-head).  Tokens past counts[b], and positions without a page, are left
+// out: nothing is written for them.
+constexpr int kAppendRows = 16;
 template <int DT, int F8>
-__global__ void __launch_bounds__(256) append_ragged_kernel(const void* __restrict__ k, const uint4* __restrict__ v,
-                                                            int64_t n_vec, int groups_per_row, int T,
+__global__ void __launch_bounds__(256) append_ragged_kernel(const uint4* __restrict__ k, const uint4* __restrict__ v,
+                                                            int blocks_per_seq, int groups_per_row, int T,
                                                             const int32_t* __restrict__ positions,
                                                             const int32_t* __restrict__ counts,
                                                             const int32_t* __restrict__ table, int stride, int cols,
                                                             int n_pages, uint8_t* __restrict__ base,
                                                             uint8_t* __restrict__ res, uint4* __restrict__ v_pool) {
   constexpr int U = 4;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i0 < n_vec; i0 += U * step) {
+  const int b = blockIdx.x / blocks_per_seq, t0 = (blockIdx.x - b * blocks_per_seq) * kAppendRows;
+  const int t1 = min(min(t0 + kAppendRows, T), counts ? counts[b] : T);
+  const int64_t pos0 = positions[b], in0 = (static_cast<int64_t>(b) * T + t0) * groups_per_row;
+  const uint32_t n = max(t1 - t0, 0) * groups_per_row;
+  for (uint32_t i0 = threadIdx.x; i0 < n; i0 += U * 256) {
     int64_t out[U];
-    float x[U][8];
-    uint4 vv[U];
+    uint4 kk[U], vv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t i = i0 + u * step;
+      const uint32_t i = i0 + u * 256;
       out[u] = -1;
-      if (i >= n_vec) continue;
-      const int64_t row = i / groups_per_row;
-      const int g = static_cast<int>(i - row * groups_per_row);
-      const int b = static_cast<int>(row / T), tt = static_cast<int>(row - static_cast<int64_t>(b) * T);
-      if (counts && tt >= counts[b]) continue;
-      const int64_t pos = static_cast<int64_t>(positions[b]) + tt;
+      if (i >= n) continue;
+      const uint32_t row = i / static_cast<uint32_t>(groups_per_row), g = i - row * groups_per_row;
+      const int64_t pos = pos0 + t0 + row;
       if (pos < 0 || pos >= static_cast<int64_t>(cols) * kPage) continue;
-      const int page = table[static_cast<int64_t>(b) * stride + pos / kPage];
+      const int page = table[static_cast<int64_t>(b) * stride + (pos >> 6)];
       if (page < 0 || page >= n_pages) continue;
-      out[u] = (static_cast<int64_t>(page) * kPage + pos % kPage) * groups_per_row + g;
-      load8<DT>(k, i * 8, x[u]);
-      vv[u] = v[i];
+      out[u] = (static_cast<int64_t>(page) * kPage + (pos & (kPage - 1))) * groups_per_row + g;
+      kk[u] = k[in0 + i];
+      vv[u] = v[in0 + i];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (out[u] < 0) continue;
       const float none[8] = {};
-      encode8<kEncFp8, DT, F8>(x[u], none, none, 0.f, base, res, out[u], true);
+      float x[8];
+      unpack8<DT>(kk[u], x);
+      encode8<kEncFp8, DT, F8>(x, none, none, 0.f, base, res, out[u], true);
       v_pool[out[u]] = vv[u];
     }
   }
@@ -643,12 +649,11 @@ extern "C" int ffa_cache_append_ragged(const void* k, const void* v, int32_t dt,
   if (!aligned16(k) || !aligned16(v) || !aligned16(base_pool) || !aligned16(residual_pool) || !aligned16(v_pool))
     return FFA_E_ALIGN;
   const int groups = HKV * D / 8;
-  const int64_t n_vec = static_cast<int64_t>(B) * T_new * groups;
-  int64_t blocks = (n_vec + 255) / 256;
-  if (blocks > 148 * 16) blocks = 148 * 16;
+  const int64_t per_seq = (static_cast<int64_t>(T_new) + kAppendRows - 1) / kAppendRows, blocks = per_seq * B;
+  if (blocks > INT32_MAX) return FFA_E_LIMIT;
 #define FFA_RAGGED(DT_, F8_)                                                                                     \
   append_ragged_kernel<DT_, F8_><<<static_cast<unsigned>(blocks), 256, 0, st>>>(                                 \
-      k, static_cast<const uint4*>(v), n_vec, groups, T_new, positions, counts, block_table, bt_stride, cols, n_pages, \
+      static_cast<const uint4*>(k), static_cast<const uint4*>(v), static_cast<int>(per_seq), groups, T_new, positions, counts, block_table, bt_stride, cols, n_pages, \
       base_pool, residual_pool, static_cast<uint4*>(v_pool))
   if (dt == FFA_BF16) { if (fp8 == FFA_E4M3) FFA_RAGGED(kBF16, kE4M3); else FFA_RAGGED(kBF16, kE5M2); }
   else { if (fp8 == FFA_E4M3) FFA_RAGGED(kF16, kE4M3); else FFA_RAGGED(kF16, kE5M2); }

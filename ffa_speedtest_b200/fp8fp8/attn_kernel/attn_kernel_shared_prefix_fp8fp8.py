@@ -13,6 +13,7 @@ import torch
 from ... import _lib
 
 PAGE = 64
+_SCALE = 1.0 / math.sqrt(128)
 
 
 class SharedPrefixWorkspace:
@@ -21,7 +22,7 @@ class SharedPrefixWorkspace:
 
     def __init__(self, B: int, HQ: int, HKV: int, device, dtype):
         self.B, self.HQ, self.HKV, self.device, self.dtype = int(B), int(HQ), int(HKV), torch.device(device), dtype
-        nbytes = _lib.lib().ffa_shared_prefix_workspace_bytes(self.B, self.HQ, self.HKV)
+        self.nbytes = nbytes = _lib.lib().ffa_shared_prefix_workspace_bytes(self.B, self.HQ, self.HKV)
         if nbytes == 0:
             raise ValueError(f"no workspace for B={B}, HQ={HQ}, HKV={HKV}: B must be 1 to 4096, HQ a multiple of HKV")
         self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -66,57 +67,60 @@ def attn_forward_decode_shared_prefix_fp8fp8(
     ``partial_out [B, HQ, 129]`` (fp32) also receives the normalised output and the base-2 log-sum-exp."""
     if not (q.is_cuda and k_fp8.is_cuda and v.is_cuda):
         raise ValueError("q, K and V must be CUDA tensors (this build has no CPU path)")
-    if q.dim() != 4 or q.shape[1] != 1 or q.shape[3] != 128:
-        raise ValueError(f"q must be [B, 1, HQ, 128], got {tuple(q.shape)}")
-    B, _, HQ, _ = q.shape
-    if k_fp8.dim() != 4 or k_fp8.shape[1] != PAGE or k_fp8.shape[3] != 128 or v.shape != k_fp8.shape:
-        raise ValueError(f"K and V must be paged pools [n_pages, 64, HKV, 128], got {tuple(k_fp8.shape)} and {tuple(v.shape)}")
-    n_pages, _, HKV, _ = k_fp8.shape
+    q_shape, k_shape = q.shape, k_fp8.shape
+    if len(q_shape) != 4 or q_shape[1] != 1 or q_shape[3] != 128:
+        raise ValueError(f"q must be [B, 1, HQ, 128], got {tuple(q_shape)}")
+    if len(k_shape) != 4 or k_shape[1] != PAGE or k_shape[3] != 128 or v.shape != k_shape:
+        raise ValueError(f"K and V must be paged pools [n_pages, 64, HKV, 128], got {tuple(k_shape)} and {tuple(v.shape)}")
+    B, HQ, n_pages, HKV = q_shape[0], q_shape[2], k_shape[0], k_shape[2]
     if HKV == 0 or HQ % HKV != 0:
         raise ValueError(f"HQ ({HQ}) must be divisible by HKV ({HKV}) for GQA")
     if HQ // HKV > 8:
         raise ValueError(f"this build supports GQA group sizes up to 8, got {HQ // HKV}")
-    fp8 = _lib.fp8_code(k_fp8.dtype)
-    v_code = _lib.float_code(v.dtype)
+    device, q_dtype, k_dtype = q.device, q.dtype, k_fp8.dtype
+    fp8, v_code = _lib.fp8_code(k_dtype), _lib.float_code(v.dtype)
     if v_code == _lib.F32:
         raise ValueError("v must be float16 or bfloat16")
     if use_fp8_residual:
         if k_residual is None:
             raise ValueError("use_fp8_residual=True requires k_residual")
-        if k_residual.shape != k_fp8.shape or k_residual.dtype != k_fp8.dtype:
+        if k_residual.shape != k_shape or k_residual.dtype != k_dtype:
             raise ValueError("k_residual must have the shape and fp8 encoding of k_fp8")
     else:
         k_residual = None
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] == 0 \
-            or block_table.stride(1) != 1 or (B > 1 and block_table.stride(0) < block_table.shape[1]):
-        raise ValueError("block_table must be an int32 tensor [B, pages] with unit stride in its last dimension")
-    NG = prefix_pages.shape[0] if prefix_pages.dim() == 1 else 0
+    table_shape = block_table.shape
+    if block_table.dtype != torch.int32 or len(table_shape) != 2 or table_shape[0] != B or table_shape[1] == 0:
+        raise ValueError("block_table must be an int32 tensor [B, pages]")
+    cols, table_stride = table_shape[1], block_table.stride(0) if B > 1 else table_shape[1]
+    if block_table.stride(1) != 1 or table_stride < cols:
+        raise ValueError("block_table must have unit stride in its last dimension and rows that do not overlap")
+    NG = prefix_pages.numel()
     for name, t, n in (("seq_lens", seq_lens, B), ("group_start", group_start, NG + 1), ("prefix_pages", prefix_pages, NG)):
         if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 vector of {n} entries")
     if not 1 <= NG <= B:
         raise ValueError(f"there must be 1 to B = {B} groups, got {NG}")
-    for name, t in (("q", q), ("k_fp8", k_fp8), ("v", v), ("k_residual", k_residual)):
+    for t in (q, k_fp8, v, k_residual):
         if t is not None and not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+            raise ValueError("q, K, residual and V must be contiguous")
     for t in (k_fp8, v, k_residual, block_table, seq_lens, group_start, prefix_pages, out, partial_out):
-        if t is not None and t.device != q.device:
-            raise ValueError(f"all tensors must be on {q.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"all tensors must be on {device}")
     if workspace is None:
-        workspace = SharedPrefixWorkspace(B, HQ, HKV, q.device, q.dtype)
-    elif not workspace.matches(B, HQ, HKV, q.device, q.dtype):
+        workspace = SharedPrefixWorkspace(B, HQ, HKV, device, q_dtype)
+    elif not workspace.matches(B, HQ, HKV, device, q_dtype):
         raise ValueError("workspace shape/device/dtype mismatch")
-    o = workspace.o if out is None else out
-    if o.shape != (B, HQ, 128) or o.dtype != q.dtype or not o.is_contiguous():
+    if out is None:
+        out = workspace.o
+    elif out.shape != (B, HQ, 128) or out.dtype != q_dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous [B, HQ, 128] tensor of q's dtype")
     if partial_out is not None and (partial_out.shape != (B, HQ, 129) or partial_out.dtype != torch.float32
                                     or not partial_out.is_contiguous()):
         raise ValueError("partial_out must be a contiguous fp32 [B, HQ, 129] tensor")
     a = _lib.FfaSharedPrefixArgs(
-        B, HQ, HKV, 128, NG, n_pages, block_table.shape[1], block_table.stride(0) if B > 1 else block_table.shape[1],
-        _lib.float_code(q.dtype), v_code, fp8, int(use_fp8_residual), 1.0 / math.sqrt(128) if scale is None else float(scale),
-        q.data_ptr(), k_fp8.data_ptr(), _lib.ptr(k_residual), v.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-        group_start.data_ptr(), prefix_pages.data_ptr(), o.data_ptr(), _lib.ptr(partial_out), workspace.scratch.data_ptr(),
-        workspace.scratch.numel())
-    _lib.enqueue(q.device, _lib.lib().ffa_decode_shared_prefix, "ffa_decode_shared_prefix", a)
-    return o
+        B, HQ, HKV, 128, NG, n_pages, cols, table_stride, _lib.float_code(q_dtype), v_code, fp8, int(use_fp8_residual),
+        _SCALE if scale is None else float(scale), q.data_ptr(), k_fp8.data_ptr(), _lib.ptr(k_residual), v.data_ptr(),
+        block_table.data_ptr(), seq_lens.data_ptr(), group_start.data_ptr(), prefix_pages.data_ptr(), out.data_ptr(),
+        _lib.ptr(partial_out), workspace.scratch.data_ptr(), workspace.nbytes)
+    _lib.enqueue(device, _lib.lib().ffa_decode_shared_prefix, "ffa_decode_shared_prefix", a)
+    return out

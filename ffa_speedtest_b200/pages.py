@@ -100,8 +100,8 @@ class PageTable:
             x = torch.tensor(list(x), dtype=torch.int32, device=self.device)
         if x.dtype != torch.int32 or x.dim() != 1 or x.device != self.device or not x.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 vector on {self.device}")
-        if x.shape[0] > self.max_seqs:
-            raise ValueError(f"{name} lists {x.shape[0]} sequences, the table has {self.max_seqs}")
+        if x.numel() > self.max_seqs:
+            raise ValueError(f"{name} lists {x.numel()} sequences, the table has {self.max_seqs}")
         return x
 
     def _pair(self, seqs: Numbers, name: str, values, value_name: str):
@@ -109,17 +109,18 @@ class PageTable:
         if isinstance(values, int):
             values = torch.full_like(seqs, values)
         values = self._list(values, value_name)
-        if values.shape != seqs.shape:
+        n = seqs.numel()
+        if values.numel() != n:
             raise ValueError(f"{name} and {value_name} must have the same length")
-        return seqs, values
+        return seqs, values, n
 
     def truncate(self, seqs: Numbers, new_lens: Union[Numbers, int]) -> None:
         """Shorten the sequences to ``new_lens`` tokens; a length above the present one changes nothing.  A sequence
         listed twice gets the smaller length."""
-        seqs, new_lens = self._pair(seqs, "seqs", new_lens, "new_lens")
-        if seqs.shape[0]:
+        seqs, new_lens, n = self._pair(seqs, "seqs", new_lens, "new_lens")
+        if n:
             _lib.enqueue(self.device, _lib.lib().ffa_pages_truncate, "ffa_pages_truncate", self._table, seqs.data_ptr(),
-                         new_lens.data_ptr(), seqs.shape[0])
+                         new_lens.data_ptr(), n)
 
     def free(self, seqs: Numbers) -> None:
         """End the sequences: ``truncate`` to zero tokens."""
@@ -128,19 +129,19 @@ class PageTable:
     def fork(self, parents: Numbers, children: Numbers) -> None:
         """Let the empty sequences ``children[i]`` begin with all tokens of ``parents[i]``, on the same pages.  No
         child may be listed twice or be a parent in the same call."""
-        parents, children = self._pair(parents, "parents", children, "children")
-        if children.shape[0]:
+        parents, children, n = self._pair(parents, "parents", children, "children")
+        if n:
             _lib.enqueue(self.device, _lib.lib().ffa_pages_fork, "ffa_pages_fork", self._table, parents.data_ptr(),
-                         children.data_ptr(), children.shape[0])
+                         children.data_ptr(), n)
 
     def extend(self, seqs: Numbers, n_new: Union[Numbers, int]) -> None:
         """Make room for ``n_new`` more tokens in each sequence (none listed twice) and add them to ``seq_lens``; the
         caller then writes the tokens.  A partly filled last page that other sequences hold too is copied to a page
         of its own first, in every pool.  All or nothing: without enough free pages no sequence changes."""
-        seqs, n_new = self._pair(seqs, "seqs", n_new, "n_new")
-        if seqs.shape[0]:
+        seqs, n_new, n = self._pair(seqs, "seqs", n_new, "n_new")
+        if n:
             _lib.enqueue(self.device, _lib.lib().ffa_pages_extend, "ffa_pages_extend", self._table, self._pool_args,
-                         seqs.data_ptr(), n_new.data_ptr(), seqs.shape[0])
+                         seqs.data_ptr(), n_new.data_ptr(), n)
 
     def compact(self, *, block_table_out: Optional[torch.Tensor] = None, refcount_out: Optional[torch.Tensor] = None) -> None:
         """Move live pages into the free ones with lower numbers, in every pool, until the live pages are the first
@@ -184,35 +185,38 @@ def append_ragged_fp8fp8(k: torch.Tensor, v: torch.Tensor, base_pool: torch.Tens
     ``[n_pages, 64, HKV, 128]``.  ``counts [B]``: tokens of each sequence that count, the rest of T_new is padding
     and is not written.  Nothing is written for positions without a page (an entry of -1, or past the table).  The
     codes are those of ``quantize_k_fp8_fp8_residual``."""
-    if not (k.is_cuda and k.dim() == 4 and k.shape[-1] == 128):
-        raise ValueError(f"k must be a CUDA tensor [B, T, HKV, 128], got {tuple(k.shape)} on {k.device}")
-    if k.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"k must be float16 or bfloat16, got {k.dtype}")
-    if v.shape != k.shape or v.dtype != k.dtype:
+    shape = k.shape
+    if not k.is_cuda or len(shape) != 4 or shape[3] != 128:
+        raise ValueError(f"k must be a CUDA tensor [B, T, HKV, 128], got {tuple(shape)} on {k.device}")
+    dtype, device, (B, T, HKV, _), pool_shape, pool_dtype = k.dtype, k.device, shape, base_pool.shape, base_pool.dtype
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"k must be float16 or bfloat16, got {dtype}")
+    if v.shape != shape or v.dtype != dtype:
         raise ValueError("v must have the shape and type of k")
-    B, T, HKV, _ = k.shape
-    if base_pool.dim() != 4 or base_pool.shape[1:] != (PAGE, HKV, 128):
-        raise ValueError(f"pools must be [n_pages, 64, {HKV}, 128], got {tuple(base_pool.shape)}")
-    fp8 = _lib.fp8_code(base_pool.dtype)
-    if residual_pool.shape != base_pool.shape or residual_pool.dtype != base_pool.dtype:
+    if len(pool_shape) != 4 or pool_shape[1:] != (PAGE, HKV, 128):
+        raise ValueError(f"pools must be [n_pages, 64, {HKV}, 128], got {tuple(pool_shape)}")
+    fp8 = _lib.fp8_code(pool_dtype)
+    if residual_pool.shape != pool_shape or residual_pool.dtype != pool_dtype:
         raise ValueError("residual_pool must have the shape and type of base_pool")
-    if v_pool.shape != base_pool.shape or v_pool.dtype != v.dtype:
+    if v_pool.shape != pool_shape or v_pool.dtype != dtype:
         raise ValueError("v_pool must have the shape of base_pool and v's type")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.stride(1) != 1 \
-            or (B > 1 and block_table.stride(0) < block_table.shape[1]):
-        raise ValueError("block_table must be an int32 tensor [B, pages] with unit stride in its last dimension")
+    table_shape = block_table.shape
+    if block_table.dtype != torch.int32 or len(table_shape) != 2 or table_shape[0] != B:
+        raise ValueError("block_table must be an int32 tensor [B, pages]")
+    cols, table_stride = table_shape[1], block_table.stride(0) if B > 1 else table_shape[1]
+    if block_table.stride(1) != 1 or table_stride < cols:
+        raise ValueError("block_table must have unit stride in its last dimension and rows that do not overlap")
     for name, t in (("positions", positions), ("counts", counts)):
         if t is not None and (t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous int32 vector of B = {B} entries")
     if not (base_pool.is_contiguous() and residual_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("pools must be contiguous")
     for t in (v, base_pool, residual_pool, v_pool, block_table, positions, counts):
-        if t is not None and t.device != k.device:
-            raise ValueError(f"all tensors must be on {k.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"all tensors must be on {device}")
     if B == 0 or T == 0:
         return
     k, v = k.contiguous(), v.contiguous()
-    _lib.enqueue(k.device, _lib.lib().ffa_cache_append_ragged, "ffa_cache_append_ragged", k.data_ptr(), v.data_ptr(),
-                 _lib.float_code(k.dtype), B, T, HKV, fp8, base_pool.data_ptr(), residual_pool.data_ptr(), v_pool.data_ptr(),
-                 base_pool.shape[0], block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1],
-                 block_table.shape[1], positions.data_ptr(), _lib.ptr(counts))
+    _lib.enqueue(device, _lib.lib().ffa_cache_append_ragged, "ffa_cache_append_ragged", k.data_ptr(), v.data_ptr(),
+                 _lib.float_code(dtype), B, T, HKV, fp8, base_pool.data_ptr(), residual_pool.data_ptr(), v_pool.data_ptr(),
+                 pool_shape[0], block_table.data_ptr(), table_stride, cols, positions.data_ptr(), _lib.ptr(counts))
