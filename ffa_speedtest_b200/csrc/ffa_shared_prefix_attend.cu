@@ -42,7 +42,7 @@ constexpr unsigned long long kWaitNs = 200ull * 1000 * 1000;
 struct Run {
   int32_t table_row, row0, rows, head;
   int32_t tok0, end, tiles;                   // first token, token that ends the item, tiles (0: no more runs)
-  int32_t small;                              // up to eight query rows
+  int32_t spread;                             // rows of a run in each 32 TMEM lanes: 8, 16 or 32; 0: up to 8 rows in all
   int64_t part;                               // first row of its partials
 };
 
@@ -177,6 +177,35 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// 16 TMEM lanes x 128 columns: registers 4 * a .. 4 * a + 3 are columns 8 * a + 2 * (lane % 4), + 1 of row lane / 4, then of
+// row lane / 4 + 8; the store of 16-bit pairs has columns 4 * a + lane % 4 of the two rows in registers 2 * a, 2 * a + 1.
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t (&r)[64], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]),
+        "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]),
+        "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]),
+        "=r"(r[63])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st_16x128(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {"
+      "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
@@ -218,6 +247,151 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// What a softmax thread knows of a query row.
+struct Row {
+  float m = -INFINITY, l = 0.f;               // reference point (log2 units), sum of the weights so far
+  float scale = 0.f;
+  int end = 0;                                // token that ends it
+  bool live = false;
+};
+// Takes a tile's maximum in.  The reference point moves only when a weight would pass 2^8: rarely, and O is rescaled only
+// then.  Returns the factor of what was summed before.
+__device__ __forceinline__ float take_maximum(Row& row, float top, bool have_o, bool& lift) {
+  top = row.live ? top * row.scale : 0.f;     // the other rows' S is whatever lay in shared memory
+  float up = 1.f;
+  if (!(top <= row.m + 8.f) || row.m == -INFINITY) {
+    const float to = top > row.m || top != top ? top : row.m;        // NaN stays and makes the row NaN
+    up = row.m == -INFINITY ? 0.f : ex2(row.m - to);
+    lift |= have_o && !(to <= row.m);
+    row.m = to;
+  }
+  return up;
+}
+
+// S of a tile to P, in place; a row to a lane.  Tile begins at token `at`; bring_down(factor) rescales O.
+template <bool VBF16, typename F>
+__device__ __forceinline__ bool softmax_32(Row& row, uint32_t s_addr, int at, bool have_o, const F& bring_down) {
+  const int lim = row.end - at;
+  const bool cut = __any_sync(0xffffffffu, lim < kSpTile);
+  uint32_t x[128];
+  float top = -INFINITY;
+  if (!cut) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_addr + 32 * c);
+    tmem_wait_ld();
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 128; i += 8)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tops[j] = max3(tops[j], __uint_as_float(x[i + j]), __uint_as_float(x[i + j + 4]));
+    top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+      uint32_t y[32];
+      tmem_ld32(y, s_addr + 32 * c);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (32 * c + i < lim) top = max3(top, __uint_as_float(y[i]), __uint_as_float(y[i]));
+    }
+  }
+  bool lift = false;
+  const float up = take_maximum(row, top, have_o, lift);
+  if (__any_sync(0xffffffffu, lift) && !bring_down(up)) return false;
+  const float neg = row.m == -INFINITY ? 0.f : -row.m;
+  float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+  if (!cut) {
+#pragma unroll
+    for (int i = 0; i < 128; i += 4) {
+      float2 a = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), row.scale, neg);
+      float2 b = fma2(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), row.scale, neg);
+      a = make_float2(ex2(a.x), ex2(a.y));
+      b = make_float2(ex2(b.x), ex2(b.y));
+      sum = add2(sum, a);
+      sum1 = add2(sum1, b);
+      x[i / 2] = pack16<VBF16>(a.x, a.y);
+      x[i / 2 + 1] = pack16<VBF16>(b.x, b.y);
+    }
+    tmem_st32(s_addr, x);
+    tmem_st32(s_addr + 32, x + 32);
+  } else {
+    // P of 32 tokens takes 16 columns, so it never reaches an S that is still to be read
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+      uint32_t y[32];
+      tmem_ld32(y, s_addr + 32 * c);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        float2 a = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), row.scale, neg);
+        a = make_float2(32 * c + i < lim ? ex2(a.x) : 0.f, 32 * c + i + 1 < lim ? ex2(a.y) : 0.f);
+        sum = add2(sum, a);
+        y[i / 2] = pack16<VBF16>(a.x, a.y);
+      }
+      tmem_st16(s_addr + 16 * c, y);
+    }
+  }
+  row.l = row.l * up + ((sum.x + sum.y) + (sum1.x + sum1.y));
+  tmem_wait_st();
+  return true;
+}
+
+// The same for up to 8 * H rows in the warp's first 16 TMEM lanes, four lanes of the warp to a row: lane i has columns
+// 8 * a + 2 * (i % 4), + 1 of rows i / 4 and i / 4 + 8.  A warp then works out 32 * H exponentials a lane, not 128.
+template <int H, bool VBF16, typename F>
+__device__ __forceinline__ bool softmax_16(Row (&row)[2], uint32_t s_addr, int at, bool have_o, const F& bring_down) {
+  const int lane = threadIdx.x & 31, col0 = 2 * (lane & 3);
+  uint32_t x[64];
+  tmem_ld_16x256(x, s_addr);
+  tmem_wait_ld();
+  const int lim0 = row[0].end - at, lim1 = H > 1 ? row[1].end - at : kSpTile;
+  if (__any_sync(0xffffffffu, min(lim0, lim1) < kSpTile)) {
+#pragma unroll
+    for (int i = 0; i < 64; ++i)
+      if (8 * (i >> 2) + (i & 1) + col0 >= ((i & 2) ? lim1 : lim0)) x[i] = 0xff800000u;
+  }
+  bool lift = false;
+  float up[2] = {1.f, 1.f};
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    float tops[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int a = 0; a < 16; ++a) tops[a & 1] = max3(tops[a & 1], __uint_as_float(x[4 * a + 2 * h]), __uint_as_float(x[4 * a + 2 * h + 1]));
+    float top = max3(tops[0], tops[1], tops[1]);
+    const float y = __shfl_xor_sync(0xffffffffu, top, 1);
+    top = max3(top, y, y);
+    const float z = __shfl_xor_sync(0xffffffffu, top, 2);
+    up[h] = take_maximum(row[h], max3(top, z, z), have_o, lift);
+  }
+  if (__any_sync(0xffffffffu, lift)) {
+    const float a = __shfl_sync(0xffffffffu, up[0], (lane & 7) * 4), b = __shfl_sync(0xffffffffu, up[1], (lane & 7) * 4);
+    if (!bring_down(lane < 8 ? a : lane < 16 ? b : 1.f)) return false;
+  }
+  uint32_t w[32];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h >= H) {
+#pragma unroll
+      for (int a = 0; a < 16; ++a) w[2 * a + h] = 0u;
+      continue;
+    }
+    const float neg = row[h].m == -INFINITY ? 0.f : -row[h].m;
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int a = 0; a < 16; ++a) {
+      float2 v = fma2(make_float2(__uint_as_float(x[4 * a + 2 * h]), __uint_as_float(x[4 * a + 2 * h + 1])), row[h].scale, neg);
+      v = make_float2(ex2(v.x), ex2(v.y));
+      sum = add2(sum, v);
+      w[2 * a + h] = pack16<VBF16>(v.x, v.y);
+    }
+    row[h].l = row[h].l * up[h] + (sum.x + sum.y);
+  }
+  tmem_st_16x128(s_addr, w);
+  tmem_wait_st();
+  return true;
 }
 
 // Sum over the CTA's threads before this one; `total` gets the sum over all.  s: one entry per warp.
@@ -403,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     };
     uint32_t q_large = 0, q_small = 0;
     auto load_q = [&](const Run& r) -> bool {
-      const bool small = r.small != 0;
+      const bool small = r.spread == 0;
       const uint32_t qb = small ? 1 + (q_small & 1) : 0, round = small ? q_small >> 1 : q_large;
       if (round > 0 && !wait(qfree(qb), (round - 1) & 1, aborted)) return false;
       if (small) ++q_small; else ++q_large;
@@ -413,10 +587,20 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       }
       if (elect()) {
         const int rows_head = p.B * p.G;
-        const uint32_t bytes = small ? 1024 : kPiece;
-        mbar_expect_tx(qfull(qb), NP * bytes);
-        for (int piece = 0; piece < NP; ++piece)
-          tma_load(q_buffer(qb) + piece * bytes, small ? &map_q8 : &map_q, 0, (piece * p.HKV + r.head) * rows_head + r.row0, qfull(qb));
+        const uint32_t dst = q_buffer(qb), step = small ? 1024 : kPiece, bar = qfull(qb);
+        if (r.spread == 32) {
+          mbar_expect_tx(bar, NP * kPiece);
+          for (int piece = 0; piece < NP; ++piece)
+            tma_load(dst + piece * step, &map_q, 0, (piece * p.HKV + r.head) * rows_head + r.row0, bar);
+        } else {
+          // eight rows at a time, eight or sixteen to a quarter of the 128
+          const int boxes = (r.rows + 7) / 8;
+          mbar_expect_tx(bar, NP * boxes * 1024);
+          for (int piece = 0; piece < NP; ++piece)
+            for (int i = 0; i < boxes; ++i)
+              tma_load(dst + piece * step + (r.spread == 16 ? (i >> 1) * 4096 + (i & 1) * 1024 : i * 4096), &map_q8, 0,
+                       (piece * p.HKV + r.head) * rows_head + r.row0 + 8 * i, bar);
+        }
       }
       __syncwarp();
       return true;
@@ -486,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
         r.tok0 = it.page0 * kPage + t0 * kSpTile;
         r.end = it.end;
         r.tiles = t1 - t0;
-        r.small = r.rows <= 8;
+        r.spread = r.rows <= 8 ? 0 : r.rows <= 32 ? 8 : r.rows <= 64 ? 16 : 32;
         r.part = sp_part_row(p, own, r.row0, r.rows, head, cta);
         if (!list(r) || !load(r)) return false;
         if (++head == p.HKV) { head = 0; ++block; }
@@ -529,11 +713,12 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     Run r;
     bool ok = true;
     while (ok && next_run(r)) {
-      const uint32_t qb = r.small ? 1 + (q_small & 1) : 0;
-      if (!wait(qfull(qb), (r.small ? q_small >> 1 : q_large) & 1, aborted)) break;
-      if (r.small) ++q_small; else ++q_large;
+      const bool small = r.spread == 0;
+      const uint32_t qb = small ? 1 + (q_small & 1) : 0;
+      if (!wait(qfull(qb), (small ? q_small >> 1 : q_large) & 1, aborted)) break;
+      if (small) ++q_small; else ++q_large;
       const uint64_t dq = desc(q_buffer(qb), 16);
-      const uint32_t q_step = (r.small ? 1024 : kPiece) >> 4;
+      const uint32_t q_step = (small ? 1024 : kPiece) >> 4;
       for (int t = 0; t < r.tiles; ++t, ++e) {
         const uint32_t s0 = pos % NS, s1 = (pos + 1) % NS, g = e & 1;
         if (!wait(full(s0), (pos / NS) & 1, aborted)) { ok = false; break; }
@@ -609,18 +794,18 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       }
     }
   } else if (warp >= 4) {
-    // ---- softmax: one query row per thread ----
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+    // ---- softmax ----
+    const int quarter = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     uint32_t e = 0, n_run = 0;
-    // a finished run whose O is still to be written
+    // a finished run whose O is still to be written, a row to a lane
     bool have_o = false, o_live = false;
     int64_t o_part = 0;
-    int o_rows = 0;
+    int o_rows = 0, o_row = 0;
     float o_m = 0.f, o_l = 0.f;
     auto write_o = [&](uint32_t o) {
       if (__any_sync(0xffffffffu, o_live)) {
-        float4* const dst = p.part_o + 32 * o_part + row;
+        float4* const dst = p.part_o + 32 * o_part + o_row;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t x[32];
@@ -632,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
               dst[static_cast<int64_t>(8 * c + i) * o_rows] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]),
                                                                           __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3]));
         }
-        if (o_live) p.part_ml[o_part + row] = make_float2(o_m, o_l);
+        if (o_live) p.part_ml[o_part + o_row] = make_float2(o_m, o_l);
       }
       fence_before();
       __syncwarp();
@@ -642,19 +827,28 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     bool ok = true;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     while (ok && next_run(r)) {
-      const bool live = row < r.rows, any_live = quarter * 32 < r.rows;
-      float m = -INFINITY, l = 0.f, scale = 0.f;
-      int end = r.end;
-      if (live) {
-        scale = p.q_scale[static_cast<int64_t>(r.head) * p.B * p.G + r.row0 + row];
-        end = min(end, p.seq_lens[(r.row0 + row) / p.G]);
+      // rows of this quarter: first, number; a row to a lane (32), or up to 8 or 16 rows with four lanes to each
+      const int per = r.spread ? r.spread : 8, first_row = quarter * per;
+      const int here = r.spread || quarter == 0 ? min(per, r.rows - first_row) : 0;
+      const bool any_live = here > 0;
+      Row row[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = per == 32 ? lane : (lane >> 2) + 8 * h;
+        row[h] = Row{};
+        row[h].live = j < here && (h == 0 || per == 16);
+        row[h].end = r.end;
+        if (row[h].live) {
+          row[h].scale = p.q_scale[static_cast<int64_t>(r.head) * p.B * p.G + r.row0 + first_row + j];
+          row[h].end = min(r.end, p.seq_lens[(r.row0 + first_row + j) / p.G]);
+        }
       }
       const uint32_t o_addr = lanes + 256 + 128 * (n_run & 1);
       for (int t = 0; t < r.tiles; ++t, ++e) {
         const uint32_t g = e & 1, s_addr = lanes + 128 * g;
         if (!wait(sfull(g), (e >> 1) & 1, aborted)) { ok = false; break; }
         fence_after();
-        // PV of the step before is done: O may be brought down, and P of that step is not needed any more
+        // PV of the step before is done: O may be brought down
         bool waited = false;
         auto pv_done = [&]() -> bool {
           if (e > 0 && !waited && !wait(sfree(g ^ 1), ((e - 1) >> 1) & 1, aborted)) return false;
@@ -662,91 +856,27 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
           fence_after();
           return true;
         };
-        if (any_live) {
-          const int lim = end - (r.tok0 + t * kSpTile);
-          const bool cut = __any_sync(0xffffffffu, lim < kSpTile);
-          uint32_t x[128];
-          float top = -INFINITY;
-          if (!cut) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_addr + 32 * c);
+        // O is rescaled by a factor per row, a row to a lane
+        auto bring_down = [&](float up) -> bool {
+          if (!pv_done()) return false;
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t y[16];
+            tmem_ld16(y, o_addr + 16 * c);
             tmem_wait_ld();
-            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 128; i += 8)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) tops[j] = max3(tops[j], __uint_as_float(x[i + j]), __uint_as_float(x[i + j + 4]));
-            top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
-          } else {
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t y[32];
-              tmem_ld32(y, s_addr + 32 * c);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (32 * c + i < lim) top = max3(top, __uint_as_float(y[i]), __uint_as_float(y[i]));
-            }
+            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * up);
+            tmem_st16(o_addr + 16 * c, y);
           }
-          top = live ? top * scale : 0.f;     // the other lanes' S is whatever lay in shared memory
-          // the reference point moves only when a weight would pass 2^8: rarely, and O is rescaled only then
-          float up = 1.f;
-          bool lift = false;
-          if (!(top <= m + 8.f) || m == -INFINITY) {
-            const float to = top > m || top != top ? top : m;      // NaN stays and makes the row NaN
-            up = m == -INFINITY ? 0.f : ex2(m - to);
-            lift = t > 0 && !(to <= m);
-            m = to;
-          }
-          if (__any_sync(0xffffffffu, lift)) {
-            if (!pv_done()) { ok = false; break; }
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-              uint32_t y[16];
-              tmem_ld16(y, o_addr + 16 * c);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * up);
-              tmem_st16(o_addr + 16 * c, y);
-            }
-          }
-          const float neg = m == -INFINITY ? 0.f : -m;
-          float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-          if (!cut) {
-#pragma unroll
-            for (int i = 0; i < 128; i += 4) {
-              float2 a = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale, neg);
-              float2 b = fma2(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale, neg);
-              a = make_float2(ex2(a.x), ex2(a.y));
-              b = make_float2(ex2(b.x), ex2(b.y));
-              sum = add2(sum, a);
-              sum1 = add2(sum1, b);
-              x[i / 2] = pack16<VBF16>(a.x, a.y);
-              x[i / 2 + 1] = pack16<VBF16>(b.x, b.y);
-            }
-            tmem_st32(s_addr, x);
-            tmem_st32(s_addr + 32, x + 32);
-          } else {
-            // P of 32 tokens takes 16 columns, so it never reaches an S that is still to be read
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t y[32];
-              tmem_ld32(y, s_addr + 32 * c);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                float2 a = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), scale, neg);
-                a = make_float2(32 * c + i < lim ? ex2(a.x) : 0.f, 32 * c + i + 1 < lim ? ex2(a.y) : 0.f);
-                sum = add2(sum, a);
-                y[i / 2] = pack16<VBF16>(a.x, a.y);
-              }
-              tmem_st16(s_addr + 16 * c, y);
-            }
-          }
-          l = l * up + ((sum.x + sum.y) + (sum1.x + sum1.y));
-          tmem_wait_st();
+          return true;
+        };
+        if (any_live) {
+          const int at = r.tok0 + t * kSpTile;
+          if (per == 32) ok = softmax_32<VBF16>(row[0], s_addr, at, t > 0, bring_down);
+          else if (per == 8) ok = softmax_16<1, VBF16>(row, s_addr, at, t > 0, bring_down);
+          else ok = softmax_16<2, VBF16>(row, s_addr, at, t > 0, bring_down);
         }
-        if (!pv_done()) { ok = false; break; }
+        if (!ok || !pv_done()) { ok = false; break; }
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(pfull(g));
@@ -757,11 +887,22 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       }
       if (!ok) break;
       have_o = true;
-      o_live = live;
+      o_live = lane < here;
       o_part = r.part;
       o_rows = r.rows;
-      o_m = m;
-      o_l = l;
+      o_row = first_row + lane;
+      if (per == 32) {
+        o_m = row[0].m;
+        o_l = row[0].l;
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          row[h].l += __shfl_xor_sync(0xffffffffu, row[h].l, 1);
+          row[h].l += __shfl_xor_sync(0xffffffffu, row[h].l, 2);
+          const float m = __shfl_sync(0xffffffffu, row[h].m, (lane & 7) * 4), l = __shfl_sync(0xffffffffu, row[h].l, (lane & 7) * 4);
+          if (lane >> 3 == h) { o_m = m; o_l = l; }
+        }
+      }
       ++n_run;
     }
     if (ok && have_o && wait(sfree((e - 1) & 1), ((e - 1) >> 1) & 1, aborted)) {
