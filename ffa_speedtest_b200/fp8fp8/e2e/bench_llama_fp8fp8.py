@@ -11,6 +11,9 @@ Arguments, modes and output lines are those of the reference driver
 through the model with a fresh cache per iteration; ``--compare`` runs the dense baseline and the FFA
 path one after the other.  Head dimension must be 128 (``hidden-size = 128 x heads``).
 
+``--samples S`` (with ``--context``) then times the same decode steps for S continuations of each of the ``--batch``
+prompts, forked from it in a ``SharedPrefixFP8Fp8Cache``.
+
 Added here: ``--context N`` fills every layer's cache with N synthetic tokens (seeded post-RoPE keys
 and values written straight into the pages, no model pass) and then times ``--decode-steps`` decode
 steps on top of it - the long-context regime the decode op is for; ``--json`` prints one JSON line
@@ -28,6 +31,7 @@ import torch
 from ...synth import make_decode_inputs
 from .fp8fp8_cache import PagedFP8Fp8Cache, resolve_fp8_dtype
 from .modeling_llama import DenseCache, LlamaConfig, LlamaForCausalLM
+from .shared_cache import SharedPrefixFP8Fp8Cache
 
 
 def parse_args(argv=None) -> argparse.Namespace:
@@ -54,6 +58,7 @@ def parse_args(argv=None) -> argparse.Namespace:
     p.add_argument("--no-fused-append", action="store_true", help="project K with torch and append the keys instead")
     p.add_argument("--context", type=int, default=0, help="synthetic tokens already in the cache before decoding")
     p.add_argument("--decode-steps", type=int, default=32, help="decode steps timed on top of --context")
+    p.add_argument("--samples", type=int, default=0, help="continuations of each prompt that share its pages (with --context)")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--json", action="store_true")
     return p.parse_args(argv)
@@ -175,8 +180,43 @@ def main(argv=None) -> dict:
             del cache
         clear_cuda()
 
+    def run_samples() -> None:
+        """S continuations of each prompt: forked, decoded for the given steps, freed again."""
+        clear_cuda()
+        P, S, steps = args.batch, args.samples, args.decode_steps
+        own = -(-(steps + 64) // 64) + 1                      # pages that a continuation writes itself
+        cache = SharedPrefixFP8Fp8Cache(P + P * S, args.kv_heads, capacity, num_layers=args.layers,
+                                        n_pages=P * -(-args.context // 64) + P * S * own, fp8_dtype=fp8_dtype, dtype=dtype, device=device)
+        _, k, v = make_decode_inputs(P, args.context, args.heads, args.kv_heads, 128, seed=args.seed + 1, dtype=dtype, device=device)
+        cache.activate(range(P))
+        cache.extend(args.context)
+        for layer in range(args.layers):
+            cache.update(k, v, layer)
+        del k, v
+        children = list(range(P, P + P * S))
+        ids = torch.randint(0, args.vocab_size, (P * S, steps), generator=gen).to(device)
+
+        def decode_steps() -> None:
+            cache.free(children)
+            cache.fork([c // S for c in range(P * S)], children)
+            cache.activate(children)
+            for t in range(steps):
+                model(ids[:, t:t + 1], past_key_values=cache, use_cache=True)
+
+        ms = benchmark_ms(decode_steps, args.iters, args.warmup)
+        cache.check()
+        tps = P * S * steps / (ms / 1000.0)
+        print(f"[FP8FP8-samples][Decode@{args.context}] {ms:.3f} ms/iter, {ms / steps:.3f} ms/token, {tps:.1f} tok/s "
+              f"({S} continuations of {P} prompts)")
+        out["samples_decode_ms_per_token"] = ms / steps
+        out["samples_decode_tok_s"] = tps
+
     t0 = time.time()
-    if args.compare:
+    if args.samples:
+        if args.samples < 0 or args.context <= 0 or args.no_residual:
+            raise ValueError("--samples takes a positive number, --context, and the residual")
+        run_samples()
+    elif args.compare:
         run_variant("Baseline", False)
         run_variant("FP8FP8", True)
     elif args.ffa_decode:

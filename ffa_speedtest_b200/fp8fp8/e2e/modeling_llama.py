@@ -15,6 +15,8 @@ What differs from the reference on purpose:
     kernel (K projection + RoPE + fp8 quantisation + scatter into the page, from the hidden state)
     and one copy kernel for V, then runs the decode op on the pools - no ``torch.cat``, no
     dequantised shadow copy of the keys;
+  * a ``SharedPrefixFP8Fp8Cache`` serves several continuations of one prompt: its sequences have positions of
+    their own, and a decode step attends to the prompt's pages once for all of them, without pruning;
   * RoPE pairs neighbouring channels (2i, 2i+1), the convention of the reference's fused K-projection
     (ffa-fp8fp8/fused_kproj_rope_fp8fp8.py:26-37), for q and k alike;
   * dense attention (prefill, and the baseline arm) is torch's scaled_dot_product_attention.
@@ -30,6 +32,7 @@ import torch.nn.functional as F
 
 from ...kproj import apply_rope, build_rope_cache
 from .fp8fp8_cache import PagedFP8Fp8Cache
+from .shared_cache import SharedPrefixFP8Fp8Cache
 
 
 @dataclass
@@ -140,7 +143,16 @@ class LlamaAttention(nn.Module):
         q = apply_rope(self.q_proj(hidden_states).view(B, T, self.num_heads, self.head_dim), cos, sin)
         v = self.v_proj(hidden_states).view(B, T, self.num_kv_heads, self.head_dim)
 
-        if isinstance(past_key_values, PagedFP8Fp8Cache):
+        if isinstance(past_key_values, SharedPrefixFP8Fp8Cache):
+            k = apply_rope(self.k_proj(hidden_states).view(B, T, self.num_kv_heads, self.head_dim), cos, sin)
+            past_key_values.update(k, v, self.layer_idx)
+            if T == 1:
+                attn = past_key_values.decode(q.contiguous(), self.layer_idx, settings.get("scale")).view(B, 1, self.num_heads, self.head_dim)
+            elif past_key_values.get_seq_length() == T:
+                attn = _dense_attention(q, k, v, causal=True)                     # prefill from empty sequences
+            else:
+                raise RuntimeError("a SharedPrefixFP8Fp8Cache serves prefill from empty sequences and single-token steps")
+        elif isinstance(past_key_values, PagedFP8Fp8Cache):
             ffa_step = T == 1 and use_ffa_decode and in_pattern
             if ffa_step and settings.get("fused_append", True) and past_key_values.use_fp8_residual:
                 # K projection + RoPE + quantisation + scatter in one kernel, straight from the hidden state
@@ -211,9 +223,16 @@ class LlamaForCausalLM(nn.Module):
     @torch.no_grad()
     def forward(self, input_ids: torch.Tensor, past_key_values=None, use_cache: bool = False) -> torch.Tensor:
         cache = past_key_values if use_cache else None
-        start = cache.get_seq_length(0) if cache is not None else 0
         x = self.embed_tokens(input_ids)
-        rope = self._rope_rows(start, input_ids.shape[1], x.dtype, x.device)
+        T = input_ids.shape[1]
+        if isinstance(cache, SharedPrefixFP8Fp8Cache):
+            cache.extend(T)
+            cos, sin = self._rope_rows(0, cache.get_seq_length(), x.dtype, x.device)
+            at = cache.positions()
+            rope = cos[at].unsqueeze(2), sin[at].unsqueeze(2)                     # [B, T, 1, D]
+        else:
+            start = cache.get_seq_length(0) if cache is not None else 0
+            rope = self._rope_rows(start, T, x.dtype, x.device)
         for layer in self.layers:
             x = layer(x, rope, cache)
         return self.lm_head(self.norm(x))

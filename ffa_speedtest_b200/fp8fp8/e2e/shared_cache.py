@@ -1,0 +1,162 @@
+"""Paged fp8 + fp8-residual cache in which sequences share the pages of a common prompt.
+
+``PagedFP8Fp8Cache`` gives every sequence its own pages and all of them one length.  Here a :class:`PageTable`
+hands pages out: ``fork`` lets a new sequence begin on the pages of a prompt, the first write into a shared open page
+copies it, ``free`` gives the pages of an ended sequence back, ``compact`` moves the pages in use to the front.  One
+table serves all layers.  A decode step appends every sequence's token at its own position and attends to shared
+pages once per group of sequences (every token counts; nothing is pruned).
+
+Sequences have numbers ``0 .. max_seqs - 1``.  ``activate`` names those that the next model calls are about, in batch
+order; sequences that were forked from one another should be next to each other in it, since a group is a stretch of
+the batch.  Lengths are known on the host as well, so that nothing here waits for the device; a call that runs out of
+pages is found by ``check()``.
+
+The reference has no counterpart (ffa-fp8fp8/e2e/fp8fp8_cache.py appends a batch of one length with ``torch.cat``).
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from ...pages import PageTable, append_ragged_fp8fp8
+from ..attn_kernel.attn_kernel_shared_prefix_fp8fp8 import SharedPrefixWorkspace, attn_forward_decode_shared_prefix_fp8fp8
+from .fp8fp8_cache import PAGE, resolve_fp8_dtype
+
+
+class SharedPrefixFP8Fp8Cache:
+    def __init__(self, max_seqs: int, num_kv_heads: int, max_seq_len: int, *, num_layers: int, n_pages: Optional[int] = None,
+                 head_dim: int = 128, fp8_dtype: Optional[torch.dtype] = None, dtype: torch.dtype = torch.bfloat16,
+                 device="cuda"):
+        if head_dim != 128:
+            raise ValueError(f"this build supports head_dim 128, got {head_dim}")
+        if num_layers <= 0:
+            raise ValueError(f"num_layers must be positive, got {num_layers}")
+        self.num_kv_heads, self.head_dim, self.num_layers, self.dtype = num_kv_heads, head_dim, num_layers, dtype
+        self.fp8_dtype = fp8_dtype or resolve_fp8_dtype(device)
+        pages_per_seq = -(-max_seq_len // PAGE)
+        self.max_seq_len = pages_per_seq * PAGE
+        shape = (n_pages or max_seqs * pages_per_seq, PAGE, num_kv_heads, head_dim)
+        self.key_base = [torch.zeros(shape, dtype=self.fp8_dtype, device=device) for _ in range(num_layers)]
+        self.key_residual = [torch.zeros(shape, dtype=self.fp8_dtype, device=device) for _ in range(num_layers)]
+        self.value = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.table = PageTable(shape[0], max_seqs, pages_per_seq, device=device,
+                               pools=[*self.key_base, *self.key_residual, *self.value])
+        self.device = self.table.device
+        self.lengths = [0] * max_seqs
+        # of every sequence: the prompt that its first pages come from, and how many of them are that prompt's
+        self._line = list(range(max_seqs))
+        self._shared = [self.max_seq_len // PAGE] * max_seqs
+        self._next_line = max_seqs
+        self._seqs: list[int] = []
+        self._new = 0
+        self._workspace: Optional[SharedPrefixWorkspace] = None
+
+    # ---- sequences ---------------------------------------------------------------------------------------
+    def _numbers(self, seqs: Sequence[int]) -> list[int]:
+        seqs = [int(s) for s in seqs]
+        if any(s < 0 or s >= len(self.lengths) for s in seqs) or len(set(seqs)) != len(seqs):
+            raise ValueError(f"sequence numbers must differ and be 0 to {len(self.lengths) - 1}, got {seqs}")
+        return seqs
+
+    def activate(self, seqs: Sequence[int]) -> None:
+        """The sequences of the next model calls, in batch order."""
+        seqs = self._numbers(seqs)
+        if not seqs:
+            raise ValueError("activate at least one sequence")
+        self._seqs = seqs
+        self._rows = torch.tensor(seqs, dtype=torch.int32, device=self.device)
+        self._slice = slice(seqs[0], seqs[0] + len(seqs)) if seqs == list(range(seqs[0], seqs[0] + len(seqs))) else None
+        self._group()
+
+    def _group(self) -> None:
+        """Stretches of the batch whose sequences come from one prompt, and the pages they have in common."""
+        start, pages = [0], []
+        for i in range(1, len(self._seqs) + 1):
+            if i == len(self._seqs) or self._line[self._seqs[i]] != self._line[self._seqs[i - 1]]:
+                members = self._seqs[start[-1]:i]
+                pages.append(min(min(self._shared[s], self.lengths[s] // PAGE) for s in members) if len(members) > 1 else 0)
+                start.append(i)
+        self._group_start = torch.tensor(start, dtype=torch.int32, device=self.device)
+        self._prefix_pages = torch.tensor(pages, dtype=torch.int32, device=self.device)
+
+    def fork(self, parents: Sequence[int], children: Sequence[int]) -> None:
+        """Let the empty sequences ``children[i]`` begin with the tokens of ``parents[i]``, on the same pages."""
+        children, parents = self._numbers(children), [int(p) for p in parents]
+        if len(parents) != len(children) or any(p < 0 or p >= len(self.lengths) or p in children for p in parents):
+            raise ValueError("fork takes one parent for each child, and no child among the parents")
+        if any(self.lengths[c] for c in children):
+            raise ValueError("the children must be empty: free them first")
+        self.table.fork(parents, children)
+        for p, c in zip(parents, children):
+            self.lengths[c], self._line[c] = self.lengths[p], self._line[p]
+            self._shared[c] = min(self._shared[p], self.lengths[p] // PAGE)
+
+    def truncate(self, seqs: Sequence[int], new_lens: Sequence[int]) -> None:
+        """Drop the tokens past ``new_lens`` (rejected drafts)."""
+        seqs, new_lens = self._numbers(seqs), [int(n) for n in new_lens]
+        if len(new_lens) != len(seqs) or any(n < 0 for n in new_lens):
+            raise ValueError("truncate takes one length for each sequence")
+        self.table.truncate(seqs, new_lens)
+        for s, n in zip(seqs, new_lens):
+            if n < self.lengths[s]:
+                self.lengths[s] = n
+                if n // PAGE < self._shared[s]:       # its later pages will not be the prompt's
+                    self._line[s], self._shared[s] = self._next_line, self.max_seq_len // PAGE
+                    self._next_line += 1
+        if self._seqs:
+            self._group()
+
+    def free(self, seqs: Sequence[int]) -> None:
+        """End the sequences and give their pages back."""
+        seqs = list(seqs)
+        self.truncate(seqs, [0] * len(seqs))
+
+    def compact(self) -> None:
+        """Move the pages in use to the front of the pools."""
+        self.table.compact()
+
+    def check(self) -> None:
+        """Raise if a call since the last check ran out of pages (waits for the device)."""
+        self.table.check()
+
+    def get_seq_length(self, layer_idx: int = 0) -> int:
+        """Tokens of the longest active sequence."""
+        return max((self.lengths[s] for s in self._seqs), default=0)
+
+    # ---- a model call --------------------------------------------------------------------------------------
+    def extend(self, n_new: int) -> None:
+        """Room for ``n_new`` more tokens of every active sequence; once per model call, before its layers."""
+        if not self._seqs:
+            raise RuntimeError("activate the sequences first")
+        if n_new <= 0 or max(self.lengths[s] for s in self._seqs) + n_new > self.max_seq_len:
+            raise ValueError(f"cache capacity {self.max_seq_len} exceeded ({self.get_seq_length()} + {n_new})")
+        self.table.extend(self._rows, n_new)
+        self._new = n_new
+        for s in self._seqs:
+            self.lengths[s] += n_new
+        if self._slice is not None:
+            self._bt, self._lens = self.table.block_table[self._slice], self.table.seq_lens[self._slice]
+        else:
+            self._bt, self._lens = self.table.block_table[self._rows], self.table.seq_lens[self._rows]
+        self._positions = self._lens - n_new
+
+    def positions(self) -> torch.Tensor:
+        """Positions ``[B, n_new]`` of the tokens of this model call."""
+        return self._positions[:, None] + torch.arange(self._new, dtype=torch.int32, device=self.device)
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
+        """Write the new tokens' post-RoPE keys (quantised) and values ``[B, n_new, HKV, 128]``."""
+        if key_states.shape != (len(self._seqs), self._new, self.num_kv_heads, self.head_dim) or value_states.shape != key_states.shape:
+            raise ValueError(f"expected [B={len(self._seqs)}, {self._new}, HKV={self.num_kv_heads}, {self.head_dim}] keys and values")
+        append_ragged_fp8fp8(key_states.to(self.dtype), value_states.to(self.dtype), self.key_base[layer_idx],
+                             self.key_residual[layer_idx], self.value[layer_idx], self._bt, self._positions)
+
+    def decode(self, q: torch.Tensor, layer_idx: int, scale: Optional[float] = None) -> torch.Tensor:
+        """Attention of ``q [B, 1, HQ, 128]`` over all tokens of its sequence -> ``[B, HQ, 128]``."""
+        ws = self._workspace
+        if ws is None or not ws.matches(q.shape[0], q.shape[2], self.num_kv_heads, q.device, q.dtype):
+            ws = self._workspace = SharedPrefixWorkspace(q.shape[0], q.shape[2], self.num_kv_heads, q.device, q.dtype)
+        return attn_forward_decode_shared_prefix_fp8fp8(
+            q, self.key_base[layer_idx], self.value[layer_idx], k_residual=self.key_residual[layer_idx], block_table=self._bt,
+            seq_lens=self._lens, group_start=self._group_start, prefix_pages=self._prefix_pages, scale=scale, workspace=ws)

@@ -1,0 +1,131 @@
+"""Prompts, forks, decode steps and page management together, through the model and the cache that it uses."""
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+from ffa_speedtest_b200.fp8fp8.e2e.modeling_llama import DenseCache, LlamaConfig, LlamaForCausalLM
+from ffa_speedtest_b200.fp8fp8.e2e.shared_cache import SharedPrefixFP8Fp8Cache
+
+pytestmark = pytest.mark.gpu
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def build(layers=2, heads=4, kv=2, vocab=97, seed=0):
+    torch.manual_seed(seed)
+    cfg = LlamaConfig(hidden_size=128 * heads, num_attention_heads=heads, num_key_value_heads=kv, num_hidden_layers=layers,
+                      max_position_embeddings=512, vocab_size=vocab)
+    return cfg, LlamaForCausalLM(cfg).to(device="cuda", dtype=torch.bfloat16).eval()
+
+
+def dense_logits(model, cfg, tokens):
+    """Logits of the last token of each of the token lists, one dense run each."""
+    out = []
+    for t in tokens:
+        cache = DenseCache(1, cfg.num_key_value_heads, 512, 128, torch.bfloat16, "cuda")
+        out.append(model(torch.tensor([t], device="cuda"), past_key_values=cache, use_cache=True)[0, -1])
+    return torch.stack(out).float()
+
+
+def close(got, ref):
+    # K is held as fp8 base + fp8 residual, as in the tests of the other cache: logits within 2 % of their largest
+    assert bool(torch.isfinite(got).all())
+    assert float((got.float() - ref).abs().max()) <= 2e-2 * max(1.0, float(ref.abs().max()))
+
+
+def test_samples_of_two_prompts_track_the_dense_model():
+    """Two prompts, three samples of the first and two of the second; one of each ends and is replaced by a fork of another
+    sample, the pages are compacted, and everything goes on."""
+    cfg, model = build()
+    g = torch.Generator().manual_seed(1)
+    draw = lambda n: torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist()
+    cache = SharedPrefixFP8Fp8Cache(9, 2, 512, num_layers=2, n_pages=40, fp8_dtype=torch.float8_e4m3fn)
+    text = {0: draw(150), 1: draw(70)}
+    for p in (0, 1):                                        # prompts of different lengths, one after the other
+        cache.activate([p])
+        logits = model(torch.tensor([text[p]], device="cuda"), past_key_values=cache, use_cache=True)[:, -1]
+        close(logits, dense_logits(model, cfg, [text[p]]))
+    cache.fork([0, 0, 0, 1, 1], [2, 3, 4, 5, 6])
+    text.update({c: list(text[p]) for p, c in zip((0, 0, 0, 1, 1), (2, 3, 4, 5, 6))})
+
+    def steps(seqs, n):
+        cache.activate(seqs)
+        for _ in range(n):
+            new = draw(len(seqs))
+            for s, x in zip(seqs, new):
+                text[s].append(x)
+            logits = model(torch.tensor(new, device="cuda")[:, None], past_key_values=cache, use_cache=True)[:, -1]
+        close(logits, dense_logits(model, cfg, [text[s] for s in seqs]))
+        assert [cache.lengths[s] for s in seqs] == cache.table.seq_lens[torch.tensor(seqs, device="cuda")].tolist()
+
+    steps([2, 3, 4, 5, 6], 1)                               # open pages are shared: all write at once
+    steps([2, 3, 4, 5, 6], 60)                              # past page boundaries
+    steps([6, 5, 0, 3], 7)                                  # the prompt itself and its sample, out of order
+    cache.free([2, 5])
+    cache.fork([3, 6], [2, 5])                              # forks of forks
+    text[2], text[5] = list(text[3]), list(text[6])
+    before = cache.table.free_pages()
+    cache.compact()
+    assert cache.table.free_pages() == before
+    live = 40 - before
+    assert int((cache.table.refcount[:live] > 0).sum()) == live
+    steps([2, 3, 4, 5, 6], 9)
+    cache.truncate([3, 4], [100, 200])                      # drafts rejected, one inside the shared pages
+    del text[3][100:], text[4][200:]
+    steps([0, 2, 3, 4], 5)
+    cache.truncate([2, 4], [64, 130])                       # while they are active: the next step must not use the old groups
+    del text[2][64:], text[4][130:]
+    for s in (0, 2, 3, 4):
+        text[s].append(5)
+    logits = model(torch.full((4, 1), 5, device="cuda"), past_key_values=cache, use_cache=True)[:, -1]
+    close(logits, dense_logits(model, cfg, [text[s] for s in (0, 2, 3, 4)]))
+    cache.check()
+
+
+def test_runs_out_of_pages_and_says_so():
+    cache = SharedPrefixFP8Fp8Cache(3, 2, 512, num_layers=1, n_pages=4)
+    cache.activate([0, 1])
+    cache.extend(128)
+    cache.check()
+    cache.extend(1)                                         # two pages more than there are
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache.check()
+
+
+def test_refusals():
+    cache = SharedPrefixFP8Fp8Cache(4, 2, 128, num_layers=1)
+    with pytest.raises(RuntimeError, match="activate"):
+        cache.extend(1)
+    for bad in ([], [0, 0], [4], [-1]):
+        with pytest.raises(ValueError):
+            cache.activate(bad)
+    cache.activate([0])
+    cache.extend(65)
+    with pytest.raises(ValueError, match="capacity"):
+        cache.extend(64)
+    with pytest.raises(ValueError, match="expected"):
+        cache.update(torch.zeros(1, 2, 2, 128, device="cuda"), torch.zeros(1, 2, 2, 128, device="cuda"), 0)
+    for parents, children in (([0], [0]), ([0, 0], [1]), ([7], [1]), ([0, 0], [1, 1])):
+        with pytest.raises(ValueError):
+            cache.fork(parents, children)
+    cache.fork([0], [1])
+    with pytest.raises(ValueError, match="empty"):
+        cache.fork([0], [1])
+    with pytest.raises(ValueError):
+        cache.truncate([0], [-1])
+    with pytest.raises(ValueError, match="num_layers"):
+        SharedPrefixFP8Fp8Cache(4, 2, 128, num_layers=0)
+    cfg, model = build(layers=1)
+    cache.activate([0])
+    with pytest.raises(RuntimeError, match="prefill from empty"):
+        model(torch.zeros(1, 2, dtype=torch.long, device="cuda"), past_key_values=cache, use_cache=True)
+
+
+def test_driver_with_samples():
+    r = subprocess.run([sys.executable, "-m", "ffa_speedtest_b200.fp8fp8.e2e.bench_llama_fp8fp8", "--context", "300", "--samples", "3",
+                        "--decode-steps", "70", "--batch", "2", "--iters", "2", "--warmup", "1", "--json"], cwd=ROOT, capture_output=True,
+                       text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "[FP8FP8-samples][Decode@300]" in r.stdout and "samples_decode_tok_s" in r.stdout
