@@ -53,24 +53,25 @@ size_t scratch_ints(int64_t n_pages, int64_t max_seqs) {
   return static_cast<size_t>(kHdrInts + n_pages + 3 * cap + max_seqs);
 }
 
-// Exclusive scan over the block's threads; `total` gets the sum.  s_warp: 33 ints.
-__device__ __forceinline__ int block_exclusive(int x, int* s_warp, int& total) {
+// Exclusive scan over the block's threads; `total` gets the sum.  s_warp: 33 entries.  64 bits: what a call asks for may be
+// far more pages than there are.
+__device__ __forceinline__ int64_t block_exclusive(int64_t x, int64_t* s_warp, int64_t& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
-  int inc = x;
+  int64_t inc = x;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, d);
+    const int64_t y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
   __syncthreads();                            // the previous scan's readers are done
   if (lane == 31) s_warp[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    const int w = lane < n_warps ? s_warp[lane] : 0;
-    int winc = w;
+    const int64_t w = lane < n_warps ? s_warp[lane] : 0;
+    int64_t winc = w;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, winc, d);
+      const int64_t y = __shfl_up_sync(0xffffffffu, winc, d);
       if (lane >= d) winc += y;
     }
     s_warp[lane] = winc - w;
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(256) fork_kernel(Table t, const int32_t* __res
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, const int32_t* __restrict__ seqs,
                                                                    const int32_t* __restrict__ n_new, int n) {
   extern __shared__ uint32_t s_bits[];
-  __shared__ int s_warp[33];
+  __shared__ int64_t s_warp[33];
   __shared__ int s_count[kPlanThreads / 32];
   begin();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, cons
     if (tid == 0) { atomicOr(t.status, FFA_PAGES_BAD_ARGUMENT); hdr[kHdrJobs] = 0; }
     return;
   }
-  int total = 0;
+  int64_t total = 0;                          // pages that the call needs
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
     const int i = i0 + tid;
     int need = 0;
@@ -206,9 +207,9 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, cons
       t.job_src()[i] = src;
       t.job_rows()[i] = rows;
     }
-    int sum;
-    const int before = block_exclusive(need, s_warp, sum);
-    if (i < n) t.first_new()[i] = total + before;
+    int64_t sum;
+    const int64_t before = block_exclusive(need, s_warp, sum);
+    if (i < n) t.first_new()[i] = static_cast<int>(min(total + before, static_cast<int64_t>(t.n_pages)));
     total += sum;
   }
   int found = 0;

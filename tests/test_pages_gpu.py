@@ -246,6 +246,36 @@ def test_captured_step():
         both(t, m, "extend", [0], [1])
 
 
+def test_more_pages_than_32_bits_count_are_refused():
+    from ffa_speedtest_b200.pages import PageTable
+    t = PageTable(50, 2500, 900000)                           # 2.25e9 pages asked for
+    seqs = torch.arange(2500, dtype=torch.int32, device="cuda")
+    t.extend(seqs, 900000 * PAGE)
+    assert t.status() == 2 and int(t.seq_lens.max()) == 0 and int(t.refcount.max()) == 0
+
+
+def test_capture_with_a_copy_between_the_calls():
+    t, m = make(30, 4, 8)
+    host = torch.tensor([70, 3], dtype=torch.int32).pin_memory()
+    new, seqs = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    zero = torch.zeros(2, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        t.truncate(seqs, zero)
+        new.copy_(host, non_blocking=True)
+        t.extend(seqs, new)
+        new.add_(1)
+        t.extend(seqs, new)
+    for a, b in ((70, 3), (1, 130)):
+        host.copy_(torch.tensor([a, b], dtype=torch.int32))
+        g.replay()
+        m.truncate([0, 3], [0, 0])
+        m.extend([0, 3], [a, b])
+        m.extend([0, 3], [a + 1, b + 1])
+        m.same_as(t)
+
+
 # ---- ragged append ------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])

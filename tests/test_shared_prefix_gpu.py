@@ -83,7 +83,8 @@ class Batch:
                 w = torch.softmax(d, -1)
                 o[b, s] = w @ v[:, h]
                 lse[b, s] = torch.logsumexp(d, -1) / math.log(2)
-                score = scale * (2.0 ** -18 * q.abs().amax(-1) * k[:, h].abs().sum(-1).amax()
+                # an error of the dot product grows with the size of the scale, whatever its sign
+                score = abs(scale) * (2.0 ** -18 * q.abs().amax(-1) * k[:, h].abs().sum(-1).amax()
                                  + 1536 * 2.0 ** -24 * (q.abs() @ k[:, h].abs().T).amax(-1))
                 weight = half_step(self.v.dtype) + 2 * score + 2.0 ** -20
                 tol[b, s] = (w @ v[:, h].abs()) * weight[:, None] + half_step(self.q.dtype) * o[b, s].abs() + 1e-7
@@ -190,6 +191,35 @@ def test_infinite_values_stay_where_they_are():
     want[4:, 5] = True
     want[:4, 9] = True
     assert torch.equal(bad, want)
+
+
+def test_scales_of_any_sign_and_a_row_that_is_not_finite():
+    for vd, sizes in ((torch.bfloat16, [3]), (torch.float16, [20])):
+        b = Batch(sizes, [3], [70], 8, 2, seed=15, vd=vd)
+        for scale in (-0.2, 0.0, 1e-6):
+            b.check(b.call(scale=scale), scale=scale)
+        want = b.call().clone()
+        b.q[1, 0, 5, 17] = math.inf
+        b.q[2, 0, 0, 3] = math.nan
+        got = b.call()
+        bad = torch.zeros(b.B, 8, dtype=torch.bool, device="cuda")
+        bad[1, 5] = bad[2, 0] = True
+        assert bool(torch.isnan(got[bad]).all()) and torch.equal(got[~bad], want[~bad])
+
+
+def test_single_sequences_in_groups_of_their_own_and_empty_groups():
+    b = Batch([1, 1, 1], [2, 0, 5], [33, 1, 200], 8, 2, seed=16)
+    b.check(b.call())
+    dev = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    b.check(b.call(group_start=dev(0, 0, 1, 3), prefix_pages=dev(7, 2, 0)))       # an empty group; two sequences that share nothing
+
+
+def test_large_batch():
+    """More sequences and groups than the kernel's threads and its near list of groups."""
+    sizes = [1, 2, 3] * 170
+    b = Batch(sizes, [i % 3 for i in range(510)], [0, 1, 5, 64, 70], 4, 1, seed=17)
+    assert b.B == 1020
+    b.check(b.call())
 
 
 def test_same_as_the_pruned_decode_that_drops_nothing():
