@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(Table t, cons
     bool bad = false;
     for (int i = tid; i < n; i += kPlanThreads) {
       const int add = n_new[i];
-      if (add < 0 || static_cast<int64_t>(t.seq_lens[seqs[i]]) + add > static_cast<int64_t>(t.cols) * kPage) bad = true;
+      if (add < 0 || t.seq_lens[seqs[i]] < 0 || static_cast<int64_t>(t.seq_lens[seqs[i]]) + add > static_cast<int64_t>(t.cols) * kPage) bad = true;
     }
     ok = !__syncthreads_or(bad);
   }

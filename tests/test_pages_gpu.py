@@ -254,6 +254,15 @@ def test_more_pages_than_32_bits_count_are_refused():
     assert t.status() == 2 and int(t.seq_lens.max()) == 0 and int(t.refcount.max()) == 0
 
 
+def test_a_length_below_zero_is_refused():
+    from ffa_speedtest_b200.pages import PageTable
+    lens = torch.tensor([0, -70], dtype=torch.int32, device="cuda")
+    bt, rc = torch.full((2, 4), -1, dtype=torch.int32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    t = PageTable.wrap(bt, lens, rc)
+    t.extend([0, 1], 1)
+    assert t.status() == 1 and lens.tolist() == [0, -70] and int(bt.max()) == -1 and int(rc.max()) == 0
+
+
 def test_capture_with_a_copy_between_the_calls():
     t, m = make(30, 4, 8)
     host = torch.tensor([70, 3], dtype=torch.int32).pin_memory()
