@@ -44,7 +44,7 @@ __device__ void split_q(const SpParams& p, int64_t row_id) {
     }
   }
   float top = 0.f;
-  bool finite = true;
+  bool finite = fabsf(p.scale_log2) < INFINITY;
 #pragma unroll
   for (int e = 0; e < 16; ++e) { top = fmaxf(top, fabsf(x[e])); finite = finite && fabsf(x[e]) < INFINITY; }
 #pragma unroll
@@ -58,7 +58,7 @@ __device__ void split_q(const SpParams& p, int64_t row_id) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = finite ? x[e] * mul : 0.f;
   if (!live) return;
-  // infinities and NaN in q make the whole row NaN; the scale stays above zero, so that the -inf of a masked token times it
+  // infinities and NaN in q or in the softmax scale make the whole row NaN; the scale stays above zero, so that the -inf of a masked token times it
   // is -inf (1e-30 times a dot product of pieces, below 2^28, is nothing in a score)
   if ((lane & 7) == 0)
     p.q_scale[row_id] = finite ? fmaxf(fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-30f) : NAN;

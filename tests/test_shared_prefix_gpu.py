@@ -207,6 +207,13 @@ def test_scales_of_any_sign_and_a_row_that_is_not_finite():
         assert bool(torch.isnan(got[bad]).all()) and torch.equal(got[~bad], want[~bad])
 
 
+def test_a_scale_that_is_not_finite():
+    b = Batch([3], [2], [40], 8, 2, seed=15)
+    for scale in (math.nan, math.inf, -math.inf):
+        assert bool(torch.isnan(b.call(scale=scale)).all())
+    b.check(b.call())
+
+
 def test_single_sequences_in_groups_of_their_own_and_empty_groups():
     b = Batch([1, 1, 1], [2, 0, 5], [33, 1, 200], 8, 2, seed=16)
     b.check(b.call())
