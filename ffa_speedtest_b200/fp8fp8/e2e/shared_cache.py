@@ -8,8 +8,8 @@ pages once per group of sequences (every token counts; nothing is pruned).
 
 Sequences have numbers ``0 .. max_seqs - 1``.  ``activate`` names those that the next model calls are about, in batch
 order; sequences that were forked from one another should be next to each other in it, since a group is a stretch of
-the batch.  Lengths are known on the host as well, so that nothing here waits for the device; a call that runs out of
-pages is found by ``check()``.
+the batch.  Lengths are known on the host as well, so that nothing here waits for the device.  A model call that runs out of
+pages writes no token; ``check()`` finds it and takes the lengths from the device again.
 
 The reference has no counterpart (ffa-fp8fp8/e2e/fp8fp8_cache.py appends a batch of one length with ``torch.cat``).
 """
@@ -47,6 +47,7 @@ class SharedPrefixFP8Fp8Cache:
         # of every sequence: the prompt that its first pages come from, and how many of them are that prompt's
         self._line = list(range(max_seqs))
         self._shared = [self.max_seq_len // PAGE] * max_seqs
+        self._held = [0] * max_seqs               # pages of it that another sequence of that prompt may count on
         self._next_line = max_seqs
         self._seqs: list[int] = []
         self._new = 0
@@ -67,7 +68,13 @@ class SharedPrefixFP8Fp8Cache:
         self._seqs = seqs
         self._rows = torch.tensor(seqs, dtype=torch.int32, device=self.device)
         self._slice = slice(seqs[0], seqs[0] + len(seqs)) if seqs == list(range(seqs[0], seqs[0] + len(seqs))) else None
+        self._new = 0
         self._group()
+
+    def _alone(self, s: int) -> None:
+        """The sequence begins a line of its own."""
+        self._line[s], self._shared[s], self._held[s] = self._next_line, self.max_seq_len // PAGE, 0
+        self._next_line += 1
 
     def _group(self) -> None:
         """Stretches of the batch whose sequences come from one prompt, and the pages they have in common."""
@@ -89,8 +96,14 @@ class SharedPrefixFP8Fp8Cache:
             raise ValueError("the children must be empty: free them first")
         self.table.fork(parents, children)
         for p, c in zip(parents, children):
-            self.lengths[c], self._line[c] = self.lengths[p], self._line[p]
-            self._shared[c] = min(self._shared[p], self.lengths[p] // PAGE)
+            self.lengths[c], pages = self.lengths[p], min(self._shared[p], self.lengths[p] // PAGE)
+            if pages == 0:
+                self._alone(c)
+                continue
+            self._line[c], self._shared[c], self._held[c] = self._line[p], pages, pages
+            self._held[p] = max(self._held[p], pages)
+        if self._seqs:
+            self._group()
 
     def truncate(self, seqs: Sequence[int], new_lens: Sequence[int]) -> None:
         """Drop the tokens past ``new_lens`` (rejected drafts)."""
@@ -101,9 +114,9 @@ class SharedPrefixFP8Fp8Cache:
         for s, n in zip(seqs, new_lens):
             if n < self.lengths[s]:
                 self.lengths[s] = n
-                if n // PAGE < self._shared[s]:       # its later pages will not be the prompt's
-                    self._line[s], self._shared[s] = self._next_line, self.max_seq_len // PAGE
-                    self._next_line += 1
+                if n // PAGE < self._held[s]:         # its next pages will not be those that the others have
+                    self._alone(s)
+        self._new = 0
         if self._seqs:
             self._group()
 
@@ -115,10 +128,21 @@ class SharedPrefixFP8Fp8Cache:
     def compact(self) -> None:
         """Move the pages in use to the front of the pools."""
         self.table.compact()
+        self._new = 0
 
     def check(self) -> None:
-        """Raise if a call since the last check ran out of pages (waits for the device)."""
-        self.table.check()
+        """Raise if a call since the last check ran out of pages (waits for the device).  The lengths are then those on
+        the device, and no sequence counts as another's sample until it is forked anew."""
+        try:
+            self.table.check()
+        except RuntimeError:
+            self.lengths = self.table.seq_lens.tolist()
+            for s in range(len(self.lengths)):        # forks since then may share less than was written down
+                self._alone(s)
+            self._new = 0
+            if self._seqs:
+                self._group()
+            raise
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         """Tokens of the longest active sequence."""
@@ -131,29 +155,35 @@ class SharedPrefixFP8Fp8Cache:
             raise RuntimeError("activate the sequences first")
         if n_new <= 0 or max(self.lengths[s] for s in self._seqs) + n_new > self.max_seq_len:
             raise ValueError(f"cache capacity {self.max_seq_len} exceeded ({self.get_seq_length()} + {n_new})")
+        at = self._slice if self._slice is not None else self._rows
+        self._positions = self.table.seq_lens[at].clone() if self._slice is not None else self.table.seq_lens[at]
         self.table.extend(self._rows, n_new)
         self._new = n_new
         for s in self._seqs:
             self.lengths[s] += n_new
-        if self._slice is not None:
-            self._bt, self._lens = self.table.block_table[self._slice], self.table.seq_lens[self._slice]
-        else:
-            self._bt, self._lens = self.table.block_table[self._rows], self.table.seq_lens[self._rows]
-        self._positions = self._lens - n_new
+        self._bt, self._lens = self.table.block_table[at], self.table.seq_lens[at]
+        self._counts = self._lens - self._positions   # 0 where there were no pages: nothing is written then
+
+    def _extended(self) -> None:
+        if self._new == 0:
+            raise RuntimeError("extend first: the active sequences or their pages changed since")
 
     def positions(self) -> torch.Tensor:
         """Positions ``[B, n_new]`` of the tokens of this model call."""
+        self._extended()
         return self._positions[:, None] + torch.arange(self._new, dtype=torch.int32, device=self.device)
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> None:
         """Write the new tokens' post-RoPE keys (quantised) and values ``[B, n_new, HKV, 128]``."""
+        self._extended()
         if key_states.shape != (len(self._seqs), self._new, self.num_kv_heads, self.head_dim) or value_states.shape != key_states.shape:
             raise ValueError(f"expected [B={len(self._seqs)}, {self._new}, HKV={self.num_kv_heads}, {self.head_dim}] keys and values")
         append_ragged_fp8fp8(key_states.to(self.dtype), value_states.to(self.dtype), self.key_base[layer_idx],
-                             self.key_residual[layer_idx], self.value[layer_idx], self._bt, self._positions)
+                             self.key_residual[layer_idx], self.value[layer_idx], self._bt, self._positions, self._counts)
 
     def decode(self, q: torch.Tensor, layer_idx: int, scale: Optional[float] = None) -> torch.Tensor:
         """Attention of ``q [B, 1, HQ, 128]`` over all tokens of its sequence -> ``[B, HQ, 128]``."""
+        self._extended()
         ws = self._workspace
         if ws is None or not ws.matches(q.shape[0], q.shape[2], self.num_kv_heads, q.device, q.dtype):
             ws = self._workspace = SharedPrefixWorkspace(q.shape[0], q.shape[2], self.num_kv_heads, q.device, q.dtype)

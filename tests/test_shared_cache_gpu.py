@@ -94,6 +94,82 @@ def test_runs_out_of_pages_and_says_so():
         cache.check()
 
 
+def test_without_pages_nothing_is_written_and_work_goes_on():
+    """A step that finds no page may not touch a token of any sequence; after the check the lengths are the device's."""
+    cfg, model = build()
+    g = torch.Generator().manual_seed(5)
+    draw = lambda n: torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist()
+    for seqs in ([0, 1, 2], [2, 0, 1]):                     # side by side in the table, and not
+        cache = SharedPrefixFP8Fp8Cache(4, 2, 512, num_layers=2, n_pages=4, fp8_dtype=torch.float8_e4m3fn)
+        text = {0: draw(100)}
+        cache.activate([0])
+        model(torch.tensor([text[0]], device="cuda"), past_key_values=cache, use_cache=True)
+        cache.fork([0, 0], [1, 2])                          # the open page is shared by three: two copies are needed, both there are
+        cache.truncate([1], [90])                           # its next token falls into a token of the others
+        text[1], text[2] = text[0][:90], list(text[0])
+        cache.fork([0], [3])
+        cache.activate(seqs)
+        pools = [x.clone() for x in cache.table.pools]
+        state = cache.table.seq_lens.clone()
+        model(torch.full((3, 1), 3, device="cuda"), past_key_values=cache, use_cache=True)          # three copies: one too many
+        with pytest.raises(RuntimeError, match="free pages"):
+            cache.check()
+        assert torch.equal(cache.table.seq_lens, state) and cache.lengths == state.tolist()
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pools, cache.table.pools))
+        cache.free([3])
+        cache.activate([1, 2])
+        for s, x in ((1, 7), (2, 9)):
+            text[s].append(x)
+        logits = model(torch.tensor([[7], [9]], device="cuda"), past_key_values=cache, use_cache=True)[:, -1]
+        cache.check()
+        close(logits, dense_logits(model, cfg, [text[1], text[2]]))
+
+
+def test_groups_through_forks_and_rejected_drafts():
+    cache = SharedPrefixFP8Fp8Cache(6, 2, 1024, num_layers=1)
+    pages = lambda: (cache._group_start.tolist(), cache._prefix_pages.tolist())
+    cache.activate([0])
+    cache.extend(200)
+    cache.activate([0, 1, 2])
+    assert pages() == ([0, 1, 2, 3], [0, 0, 0])
+    cache.fork([0, 0], [1, 2])                              # while they are active
+    assert pages() == ([0, 3], [3])
+    cache.extend(70)
+    cache.truncate([0, 1, 2], [210, 201, 199])              # behind what was forked: still one prompt
+    assert pages() == ([0, 3], [3])
+    cache.truncate([0], [190])                              # into it: the other two have its third page, it will have another
+    assert pages() == ([0, 1, 3], [0, 3])
+    cache.free([1, 2])
+    cache.activate([1])
+    cache.extend(130)                                       # a prompt in the place of a sample
+    cache.fork([1], [2])
+    cache.activate([1, 2, 0])
+    assert pages() == ([0, 2, 3], [2, 0])
+    cache.activate([3])
+    cache.extend(20)
+    cache.fork([3], [4])                                    # no full page to share; both go on by themselves
+    cache.activate([3, 4])
+    cache.extend(300)
+    cache.fork([4], [5])
+    cache.activate([3, 4, 5])
+    assert pages() == ([0, 1, 3], [0, 5])
+    cache.check()
+
+
+def test_decode_needs_an_extend_after_the_pages_changed():
+    cache = SharedPrefixFP8Fp8Cache(4, 2, 256, num_layers=1)
+    q, k = torch.zeros(1, 1, 4, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16, device="cuda")
+    for change in (lambda: cache.activate([0]), lambda: cache.truncate([0], [1]), cache.compact):
+        cache.activate([0])
+        cache.extend(1)
+        cache.update(k, k, 0)
+        cache.decode(q, 0)
+        change()
+        for call in (lambda: cache.decode(q, 0), lambda: cache.update(k, k, 0), cache.positions):
+            with pytest.raises(RuntimeError, match="extend first"):
+                call()
+
+
 def test_refusals():
     cache = SharedPrefixFP8Fp8Cache(4, 2, 128, num_layers=1)
     with pytest.raises(RuntimeError, match="activate"):
