@@ -12,15 +12,25 @@
 //
 // Bound: per 128 tokens and kv-head 64 KiB arrive, 2840 clocks of an SM's share of HBM at 1.9 GHz.  The tensor core needs
 // 16 (24) + 8 MMAs of 64 clocks a step.  The softmax of a row takes 128 exponentials, 1024 clocks of the special-function
-// unit of a quarter of the SM, and some 1000 clocks around them (exponentials by a polynomial on the FMA units were tried:
-// half of them so made a step 600 clocks longer).
+// unit of a quarter of the SM, and some 600 clocks around them (exponentials by a polynomial on the FMA units were tried:
+// half of them so made a step 600 clocks longer).  Measured, with the kernels before and after (bf16, 8 kv-heads, 4 query
+// heads to each): 8 samples of 32K tokens 42 us for 147 MB, of which 4 until the first tile and 5 for the merge; 16
+// sequences that share nothing 89 us for 400 MB, 4.5 TB/s; 64 samples of 128K 311 us: 256 rows are two units, each of
+// which reads the prompt, 1353 MB at 5.6 TB/s and an SM clock that the power limit holds at 1.56 GHz.
+// One unit of 256 rows (an S and an O for each half, two softmax groups) was tried: it halves the bytes, but leaves one S
+// buffer to a half, so that S, softmax and P V follow one another: the same time there, 1 to 7 us more elsewhere.
+// S given back as soon as it is in registers, P in columns of its own (then there is room for one O only): 3 us more in
+// the smaller cases, nothing gained in the largest.
 //
 // Warps: 0 lists the runs and loads q, K and V; 1 issues the MMAs of S, 2 those of O (two warps, so that the waits of one
 // do not keep the other's from the tensor core); 4-7 softmax (TMEM lanes 32 * (warp % 4)).
 // A ring of 16 KiB slots holds, tile after tile, K base, K residual, V of the first and of the second page.  S has two
 // buffers, for even and odd steps: S of step i+1 is made while the softmax of step i runs.  P overwrites the S that it came
 // from.  O has two buffers, for even and odd runs: a run's O is written out while the next run has begun.
-// Runs of up to eight query rows (a sequence's own pages) have two small q buffers, larger ones one of 256 rows.
+// Runs of up to eight query rows (a sequence's own pages) have two small q buffers, larger ones one of 128 rows.  Up to 32
+// (64) rows are spread over the four quarters of the TMEM lanes, eight (sixteen) to each, so that all four softmax warps
+// have work, and there four lanes share a row (softmax_16): 32 (64) exponentials a lane and not 128.  16 sequences that
+// share nothing, sustained: 94.3 -> 92.5 us.
 //
 // The line of costs does not depend on the kernel that splits q, nor do K and V: both are begun while that one runs.
 //
@@ -974,7 +984,7 @@ int launch(const SpParams& p, const CUtensorMap* maps, cudaStream_t st) {
     if (e != cudaSuccess) return note_cuda_error(e, "cudaFuncSetAttribute(sp_attend_mma)");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  // set up while the plan still runs; it waits for the plan's end before it reads
+  // set up while the kernel that splits q still runs; it waits for that one's end before it reads its pieces
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.n_ctas));
   cfg.blockDim = dim3(kThreads);

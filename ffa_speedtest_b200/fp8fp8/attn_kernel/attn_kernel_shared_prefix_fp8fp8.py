@@ -63,7 +63,8 @@ def attn_forward_decode_shared_prefix_fp8fp8(
 
     Sequences ``group_start[g] .. group_start[g+1] - 1`` share their first ``prefix_pages[g]`` pages: those are taken
     from the table row of the group's first sequence.  ``seq_lens`` counts all tokens of a sequence, shared ones
-    included; a sequence of length 0 gives zeros.  Lengths and groups are read on the device when the kernels run.
+    included; a sequence of length 0 gives zeros, one that is shorter than its group's prefix sees its own tokens only (V
+    of the others has to be finite there).  Lengths and groups are read on the device when the kernels run.
     ``partial_out [B, HQ, 129]`` (fp32) also receives the normalised output and the base-2 log-sum-exp."""
     if not (q.is_cuda and k_fp8.is_cuda and v.is_cuda):
         raise ValueError("q, K and V must be CUDA tensors (this build has no CPU path)")

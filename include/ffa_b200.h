@@ -324,9 +324,12 @@ int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* pools, int3
  * Sequence b of group g (group_start[g] <= b < group_start[g + 1]) has seq_lens[b] tokens; tokens below
  * 64 * prefix_pages[g] are in the pages that the table row of the group's FIRST sequence names, the others in those of
  * its own row.  A sequence shorter than the prefix sees its first seq_lens[b] tokens; one of length 0 gives zeros.  A
- * sequence outside every group has no shared part, nor has any if the bounds do not ascend.  All of this is device memory and is read by the kernels, so a
- * captured call follows it.  Entries outside 0 .. n_pages - 1 read as zero keys and values.  The reference has no
- * counterpart (its sequences share nothing).
+ * sequence outside every group has no shared part, nor has any if the bounds do not ascend.  All of this is device
+ * memory and is read by the kernels, so a captured call follows it.  Entries outside 0 .. n_pages - 1 read as zero keys
+ * and values.  V that a sequence of a group does not see but another one does (a sequence shorter than the prefix) has
+ * to be finite.  A row of q that is not finite, or an sm_scale that is not, gives NaN.  At most 4096 sequences; a batch
+ * whose table could hold more work than 2^31 units (4 per 128 tokens, kv-head and block of 128 query rows) gives
+ * FFA_E_LIMIT.  The reference has no counterpart (its sequences share nothing).
  */
 typedef struct FfaSharedPrefixArgs {
   int32_t B, HQ, HKV;       /* B <= 4096, HQ / HKV <= 8                                              */
