@@ -29,8 +29,9 @@
 // from.  O has two buffers, for even and odd runs: a run's O is written out while the next run has begun.
 // Runs of up to eight query rows (a sequence's own pages) have two small q buffers, larger ones one of 128 rows.  Up to 32
 // (64) rows are spread over the four quarters of the TMEM lanes, eight (sixteen) to each, so that all four softmax warps
-// have work, and there four lanes share a row (softmax_16): 32 (64) exponentials a lane and not 128.  16 sequences that
-// share nothing, sustained: 94.3 -> 92.5 us.
+// have work, and there four lanes share a row (softmax_16): 32 (64) exponentials a lane and not 128.  Up to 64 rows the
+// MMAs have M = 64, which takes as long as 128 but less power, and the clock rises.  16 sequences that share nothing, under
+// sustained load: 94.3 us with a row to a lane and M = 128, 92.5 spread, 83.3 with M = 64.
 //
 // The line of costs does not depend on the kernel that splits q, nor do K and V: both are begun while that one runs.
 //
@@ -132,9 +133,10 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
   return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 |
          static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
 }
-// Instruction descriptor: fp32 accumulator, A and B formats, B transposed (MN-major) or not, M = N = 128.
-__host__ __device__ constexpr uint32_t instr(uint32_t a, uint32_t b, uint32_t b_mn) {
-  return (1u << 4) | (a << 7) | (b << 10) | (b_mn << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+// Instruction descriptor: fp32 accumulator, A and B formats, B transposed (MN-major) or not, N = 128, M = 128 or 64.  With
+// M = 64 rows 16 * i .. 16 * i + 15 are the first 16 lanes of quarter i of the TMEM lanes.
+__host__ __device__ constexpr uint32_t instr(uint32_t a, uint32_t b, uint32_t b_mn, uint32_t m) {
+  return (1u << 4) | (a << 7) | (b << 10) | (b_mn << 16) | ((128u >> 3) << 17) | ((m >> 4) << 24);
 }
 __device__ __forceinline__ void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -603,12 +605,12 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
           for (int piece = 0; piece < NP; ++piece)
             tma_load(dst + piece * step, &map_q, 0, (piece * p.HKV + r.head) * rows_head + r.row0, bar);
         } else {
-          // eight rows at a time, eight or sixteen to a quarter of the 128
+          // eight rows at a time, eight or sixteen to a quarter of the 64
           const int boxes = (r.rows + 7) / 8;
           mbar_expect_tx(bar, NP * boxes * 1024);
           for (int piece = 0; piece < NP; ++piece)
             for (int i = 0; i < boxes; ++i)
-              tma_load(dst + piece * step + (r.spread == 16 ? (i >> 1) * 4096 + (i & 1) * 1024 : i * 4096), &map_q8, 0,
+              tma_load(dst + piece * step + i * (r.spread == 16 ? 1024 : 2048), &map_q8, 0,
                        (piece * p.HKV + r.head) * rows_head + r.row0 + 8 * i, bar);
         }
       }
@@ -717,7 +719,6 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     }
   } else if (warp == 1) {
     // ---- S = q K^T ----
-    const uint32_t idesc = instr(0, p.fp8 == FFA_E4M3 ? 0 : 1, 0);
     uint32_t pos = 0, e = 0;                  // slots of the tiles before the present one, steps before it
     uint32_t q_large = 0, q_small = 0;        // runs with the large or a small q buffer
     Run r;
@@ -727,6 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       const uint32_t qb = small ? 1 + (q_small & 1) : 0;
       if (!wait(qfull(qb), (small ? q_small >> 1 : q_large) & 1, aborted)) break;
       if (small) ++q_small; else ++q_large;
+      const uint32_t idesc = instr(0, p.fp8 == FFA_E4M3 ? 0 : 1, 0, r.spread == 32 ? 128 : 64);
       const uint64_t dq = desc(q_buffer(qb), 16);
       const uint32_t q_step = (small ? 1024 : kPiece) >> 4;
       for (int t = 0; t < r.tiles; ++t, ++e) {
@@ -759,12 +761,12 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     }
   } else if (warp == 2) {
     // ---- O += P V ----
-    const uint32_t idesc = instr(VBF16 ? 1 : 0, VBF16 ? 1 : 0, 1);
     uint32_t pos = 0, e = 0, n_run = 0;
     Run r;
     bool ok = true;
     while (ok && next_run(r)) {
       const uint32_t o = n_run & 1, d = tmem + 256 + 128 * o;
+      const uint32_t idesc = instr(VBF16 ? 1 : 0, VBF16 ? 1 : 0, 1, r.spread == 32 ? 128 : 64);
       if (n_run >= 2 && !wait(ofree(o), ((n_run >> 1) - 1) & 1, aborted)) break;
       ++n_run;
       for (int t = 0; t < r.tiles && ok; ++t, ++e) {
