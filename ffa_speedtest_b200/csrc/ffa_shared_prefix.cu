@@ -90,17 +90,24 @@ __global__ void __launch_bounds__(kSplitThreads) sp_split_kernel(const __grid_co
   split_q(p, static_cast<int64_t>(blockIdx.x) * (kSplitThreads / 8) + threadIdx.x / 8);
 }
 
-// One block per sequence and kv-head: kMergeWays x (G rows x 32 groups of four channels).  The partials of a row - of the
-// shared pages, then of its own, in the order of the line - are dealt out in turn to the ways, so that many loads are in
-// flight together, and added up in a fixed order.  A row without a token gives zeros and a log-sum-exp of -inf.
-// Bound by latency: a chain of three loads and two exchanges.  At 8 samples of 32K (5 MB of partials, some 20 to a row)
-// 4.8 us from the end of the attention; with 256 threads and no ways 1 to 2 us more.
+// Blocks of a sequence and kv-head and a slice of the channels: 128 * G threads are ways x (G rows x groups of four
+// channels).  The partials of a row - of the shared pages, then of its own, in the order of the line - are dealt out in
+// turn to the ways, so that many loads are in flight together, and added up in a fixed order.  A row without a token gives
+// zeros and a log-sum-exp of -inf.  Bound by latency: a chain of three loads and two exchanges, then some 20 partials a row.
+//
+// The blocks are given out as SMs fall free of the attention, as many to an SM as it can hold.  So few sequences are cut
+// into slices, and a block asks for a share of shared memory that leaves no room for more of them than an even spread needs.
+// Replayed as a graph: 10 sequences of one head each over 49K shared tokens 52.8 -> 20 us (their blocks had all gone to the
+// SM that finished first), 8 samples of 20K 47.5 -> 40; over 28 batches of mixed shapes 34.3 -> 31.5 in geometric mean.
 constexpr int kMergeWays = 4;
+template <int SLICES>
 __global__ void __launch_bounds__(1024) sp_merge_kernel(const __grid_constant__ SpParams p) {
-  extern __shared__ float4 s_o[];             // [ways][G * 32], then [ways][G] maximum and sum
+  extern __shared__ float4 s_o[];             // [threads], then [ways][G] maximum and sum
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int b = blockIdx.x / p.HKV, head = blockIdx.x % p.HKV, lane_row = threadIdx.x % (32 * p.G), way = threadIdx.x / (32 * p.G);
-  const int c4 = lane_row / p.G, g = lane_row % p.G;
+  constexpr int ways = kMergeWays * SLICES, channels = 32 / SLICES;
+  const int slice = blockIdx.x % SLICES, pair = blockIdx.x / SLICES, b = pair / p.HKV, head = pair % p.HKV, per_way = channels * p.G;
+  const int lane_row = threadIdx.x % per_way, way = threadIdx.x / per_way;
+  const int c4 = slice * channels + lane_row / p.G, g = lane_row % p.G;
   const SpSequence me = p.sequences[b];
   const int W = p.hdr[0];
   const bool gave_up = p.hdr[1] != 0;
@@ -129,12 +136,12 @@ __global__ void __launch_bounds__(1024) sp_merge_kernel(const __grid_constant__ 
   float m = -INFINITY, l = 0.f, o[4] = {};
   constexpr int U = 6;
 #pragma unroll 1
-  for (int k0 = way; k0 < total; k0 += U * kMergeWays) {
+  for (int k0 = way; k0 < total; k0 += U * ways) {
     float4 x[U];
     float2 ml[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * kMergeWays;
+      const int k = k0 + u * ways;
       ml[u] = make_float2(-INFINITY, 0.f);
       x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k < total) {
@@ -159,21 +166,21 @@ __global__ void __launch_bounds__(1024) sp_merge_kernel(const __grid_constant__ 
     }
     m = top;
   }
-  float2* const s_ml = reinterpret_cast<float2*>(s_o + kMergeWays * 32 * p.G);
+  float2* const s_ml = reinterpret_cast<float2*>(s_o + blockDim.x);
   s_o[threadIdx.x] = make_float4(o[0], o[1], o[2], o[3]);
-  if (c4 == 0) s_ml[way * p.G + g] = make_float2(m, l);
+  if (lane_row < p.G) s_ml[way * p.G + g] = make_float2(m, l);
   __syncthreads();
   if (way != 0) return;
   float top = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kMergeWays; ++w) top = fmaxf(top, s_ml[w * p.G + g].x);
+  for (int w = 0; w < ways; ++w) top = fmaxf(top, s_ml[w * p.G + g].x);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f, y[4] = {};
 #pragma unroll
-  for (int w = 0; w < kMergeWays; ++w) {
+  for (int w = 0; w < ways; ++w) {
     const float2 ml = s_ml[w * p.G + g];
     const float f = exp2f(ml.x - ref);
-    const float4 x = s_o[w * 32 * p.G + lane_row];
+    const float4 x = s_o[w * per_way + lane_row];
     sum += ml.y * f;
     y[0] += x.x * f; y[1] += x.y * f; y[2] += x.z * f; y[3] += x.w * f;
   }
@@ -209,6 +216,20 @@ int sm_count() {
     n[dev] = cudaDeviceGetAttribute(&x, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && x > 0 ? x : 148;
   }
   return n[dev];
+}
+
+constexpr size_t kMergeSmem = 228 * 1024;     // of an SM
+int allow_merge_smem() {
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !configured[dev]) {
+    for (void (*f)(SpParams) : {sp_merge_kernel<1>, sp_merge_kernel<2>, sp_merge_kernel<4>}) {
+      const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMergeSmem - 1024);
+      if (e != cudaSuccess) return note_cuda_error(e, "cudaFuncSetAttribute(sp_merge)");
+    }
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  return FFA_OK;
 }
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
@@ -293,16 +314,23 @@ extern "C" int ffa_decode_shared_prefix(const FfaSharedPrefixArgs* a, ffa_stream
   if (rc) return rc;
   if ((rc = launch_sp_attend(p, st))) return rc;
   // the merge's blocks are set up while the attention still runs; they wait for its end before they read
+  const int64_t pairs = static_cast<int64_t>(p.B) * p.HKV;
+  const int slices = pairs * 4 <= p.n_ctas ? 4 : pairs * 2 <= p.n_ctas ? 2 : 1;
+  const int64_t per_sm = (pairs * slices + p.n_ctas - 1) / p.n_ctas;
+  const size_t need = kMergeWays * p.G * (32 * sizeof(float4) + slices * sizeof(float2));
+  const size_t share = per_sm > 4 ? 0 : kMergeSmem / per_sm - 1024;           // 1 KiB of each block is the system's
+  void (*const merge)(SpParams) = slices == 4 ? sp_merge_kernel<4> : slices == 2 ? sp_merge_kernel<2> : sp_merge_kernel<1>;
+  if ((rc = allow_merge_smem())) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.B) * p.HKV);
+  cfg.gridDim = dim3(static_cast<unsigned>(pairs * slices));
   cfg.blockDim = dim3(kMergeWays * 32 * p.G);
-  cfg.dynamicSmemBytes = kMergeWays * p.G * (32 * sizeof(float4) + sizeof(float2));
+  cfg.dynamicSmemBytes = share > need ? share : need;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sp_merge_kernel, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, merge, p);
   return e == cudaSuccess ? FFA_OK : note_cuda_error(e, "ffa_decode_shared_prefix (merge)");
 }

@@ -19,8 +19,9 @@ constexpr int kSpTile = 128;                  // tokens of a tile: two pages
 constexpr int kSpRows = 128;                  // query rows of a unit, at most
 constexpr int kSpMaxCtas = 148;
 
-// Costs, in quarters of a tile: beginning a unit (q, the first loads' latency, its partials), and a tile.
-constexpr int kSpBegin = 4, kSpTileCost = 4;
+// Costs, in quarters of a tile: beginning a unit (q, the first loads' latency, its partials), and a tile.  Over 28 batches
+// of mixed shapes 4, 5, 6 and 8 for the first gave 34.6, 34.3, 34.1 and 34.4 us in geometric mean.
+constexpr int kSpBegin = 6, kSpTileCost = 4;
 
 // where the merge finds the partials of a sequence's rows: the places of its item and of its group's on the line
 struct SpSequence {
