@@ -14,9 +14,9 @@
 // 16 (24) + 8 MMAs of 64 clocks a step.  The softmax of a row takes 128 exponentials, 1024 clocks of the special-function
 // unit of a quarter of the SM, and some 600 clocks around them (exponentials by a polynomial on the FMA units were tried:
 // half of them so made a step 600 clocks longer).  Measured, with the kernels before and after (bf16, 8 kv-heads, 4 query
-// heads to each): 8 samples of 32K tokens 42 us for 147 MB, of which 4 until the first tile and 5 for the merge; 16
-// sequences that share nothing 89 us for 400 MB, 4.5 TB/s; 64 samples of 128K 311 us: 256 rows are two units, each of
-// which reads the prompt, 1353 MB at 5.6 TB/s and an SM clock that the power limit holds at 1.56 GHz.
+// heads to each): 8 samples of 32K tokens 39 us for 147 MB, of which 4 until the first tile; 16 sequences that share
+// nothing 83 us for 400 MB, 4.8 TB/s; 64 samples of 128K 312 us (243 without a load before it): 256 rows are two units,
+// each of which reads the prompt, 1353 MB at 5.6 TB/s and an SM clock that the power limit holds at 1.6 GHz and below.
 // One unit of 256 rows (an S and an O for each half, two softmax groups) was tried: it halves the bytes, but leaves one S
 // buffer to a half, so that S, softmax and P V follow one another: the same time there, 1 to 7 us more elsewhere.
 // S given back as soon as it is in registers, P in columns of its own (then there is room for one O only): 3 us more in
