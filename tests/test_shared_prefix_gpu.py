@@ -121,6 +121,20 @@ def test_against_the_definition(case, qd, vd, fp8):
     b.check(b.call())
 
 
+@pytest.mark.parametrize("rows", [7, 8, 9, 16, 31, 32, 33, 63, 64, 65, 127, 128, 129])
+def test_numbers_of_query_rows(rows):
+    """Around the numbers of rows where the way they lie in the tile changes, one head and many partials to a row."""
+    b = Batch([rows], [301], [0, 1, 130], 1, 1, seed=rows)
+    b.check(b.call())
+
+
+@pytest.mark.parametrize("B", [1, 4, 5, 9, 10, 18, 19, 37, 74, 75])
+def test_numbers_of_sequences(B):
+    """Around the numbers where the merge is cut differently (37, 74 and 148 heads of sequences, and two and more to an SM)."""
+    b = Batch([B - B // 2] + [B // 2] * (B > 1), [40, 25][:1 + (B > 1)], [70, 0, 260], 16, 8, seed=B)
+    b.check(b.call())
+
+
 @pytest.mark.parametrize("qd", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("vd", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("fp8", [E4, E5])
