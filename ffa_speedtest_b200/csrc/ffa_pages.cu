@@ -24,7 +24,8 @@ constexpr int kChunk = kCopyThreads * 16 * 4; // bytes a block of the copy kerne
 // scratch: header, then arrays of ints
 enum { kHdrOk = 0, kHdrJobs = 1, kHdrLive = 2, kHdrArrive = 3, kHdrInts = 16 };
 
-__device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPage - 1) / kPage; }
+// Any int: a new length may be as large as the caller likes, and tokens + 63 would wrap to a page far in front of the row.
+__device__ __forceinline__ int pages_of(int tokens) { return tokens / kPage + (tokens % kPage > 0); }
 
 // Every kernel here is launched while the one before it in the stream may still run (programmatic dependent launch): it
 // is set up meanwhile and waits for that one's end before it reads anything.

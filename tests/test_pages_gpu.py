@@ -263,6 +263,21 @@ def test_a_length_below_zero_is_refused():
     assert t.status() == 1 and lens.tolist() == [0, -70] and int(bt.max()) == -1 and int(rc.max()) == 0
 
 
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 63, 2 ** 31 - 64, 200, 130])
+def test_a_new_length_above_the_present_one_changes_nothing(length):
+    from ffa_speedtest_b200.pages import PageTable
+    t, m = make(12, 4, 6)
+    both(t, m, "extend", [1, 2], [130, 64])
+    both(t, m, "truncate", [1, 2, 0], [length, length, length])
+    both(t, m, "truncate", [1, 1], [length, 70])              # the smaller of two
+    t.check()
+    # a wrapped length that the table cannot hold: shortened, and only the row's own columns are touched
+    bt, rc = torch.tensor([[0, 1], [2, -1]], dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([2 ** 31 - 1, 64], dtype=torch.int32, device="cuda")
+    PageTable.wrap(bt, lens, rc).truncate([0], [64])
+    assert bt.tolist() == [[0, -1], [2, -1]] and lens.tolist() == [64, 64] and rc.tolist() == [1, 0, 1]
+
+
 def test_capture_with_a_copy_between_the_calls():
     t, m = make(30, 4, 8)
     host = torch.tensor([70, 3], dtype=torch.int32).pin_memory()
