@@ -568,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
 
   const uint32_t nk = p.r ? 2 : 1;            // slots of a K tile
   uint32_t issued = 0;                        // warp 0: slots filled so far
+  uint32_t q_large = 0, q_small = 0;          // warps 0 and 1: runs so far with the large and with a small q buffer
   if (idle) {
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
   } else if (warp == 0) {
@@ -587,7 +588,6 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       ++listed;
       return true;
     };
-    uint32_t q_large = 0, q_small = 0;
     auto load_q = [&](const Run& r) -> bool {
       const bool small = r.spread == 0;
       const uint32_t qb = small ? 1 + (q_small & 1) : 0, round = small ? q_small >> 1 : q_large;
@@ -720,7 +720,6 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   } else if (warp == 1) {
     // ---- S = q K^T ----
     uint32_t pos = 0, e = 0;                  // slots of the tiles before the present one, steps before it
-    uint32_t q_large = 0, q_small = 0;        // runs with the large or a small q buffer
     Run r;
     bool ok = true;
     while (ok && next_run(r)) {
@@ -926,8 +925,13 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   __syncwarp();
   __syncthreads();
   if (*aborted) {
-    // what is still on its way must land before the CTA's memory is given up
+    // what is still on its way must land before the CTA's memory is given up: slots of the ring, and each q buffer's last load
     if (warp == 0) {
+      if (q_large > 0) wait_lane(qfull(0), (q_large - 1) & 1, aborted + 1);
+      for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t n = (q_small + 1 - i) / 2;                                  // the small buffers take turns
+        if (n > 0) wait_lane(qfull(1 + i), (n - 1) & 1, aborted + 1);
+      }
       for (uint32_t n = issued > NS ? issued - NS : 0; n < issued; ++n) wait_lane(full(n % NS), (n / NS) & 1, aborted + 1);
       if (lane == 0) { p.hdr[1] = 1; atomicExch(p.status, 1); }
     } else if (warp == 1) {
