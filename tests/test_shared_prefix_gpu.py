@@ -193,6 +193,25 @@ def test_growing_scores_and_one_loud_token():
     assert float((b.call().float() - 1).abs().max()) <= half_step(torch.bfloat16)
 
 
+@pytest.mark.parametrize("vd", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gap", [17, 25])
+@pytest.mark.parametrize("sizes,prefix,own", [([1, 1], 0, 2048), ([12], 32, 10), ([40], 32, 10), ([100], 32, 10)])
+def test_one_token_far_above_many(sizes, prefix, own, gap, vd):
+    """A first token whose weight is 2^gap times that of the others and whose V is zero: what the others add up to is the
+    output, whatever the type that weights are held in.  Ways of all layouts of the query rows."""
+    b = Batch(sizes, [prefix] * len(sizes), [own], 1, 1, qd=torch.float32, vd=vd, seed=gap + sum(sizes))
+    u = 2 * torch.randn(D, generator=torch.Generator(device="cuda").manual_seed(gap), device="cuda")
+    b.q = (u * (1 + 0.01 * torch.randn(b.B, 1, 1, D, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")))
+    b.k = (0.02 * b.k.float()).to(b.k.dtype)
+    b.r.zero_()
+    b.v = b.v.abs() + 0.5
+    for i in set(b.first) if prefix else range(b.B):
+        page = int(b.table[i, 0])
+        b.k[page, 0, 0] = (gap * math.log(2) * math.sqrt(D) * u / u.square().sum()).to(b.k.dtype)
+        b.v[page, 0] = 0
+    b.check(b.call())
+
+
 def test_infinite_values_stay_where_they_are():
     b = Batch([2], [2], [30], 8, 2, seed=8)
     page = int(b.table[1, 2])                                # a page of the second sequence alone
