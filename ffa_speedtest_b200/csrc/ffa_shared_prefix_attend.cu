@@ -85,17 +85,22 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
-// A lane's wait for the phase of this parity; gives up after kWaitNs, or when another warp of the CTA has.
-__device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, int* abort_flag) {
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// A lane's wait for the phase of this parity; gives up after kWaitNs, or when another warp of the CTA has.  What a wait that
+// does not end at once needs is a call of its own: inlined at every wait the code no longer fits where instructions are held.
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, int* abort_flag) {
   unsigned long long t0 = 0;
+#pragma unroll 1
   for (int spin = 0;; ++spin) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
+    if (try_wait(bar, parity)) return true;
     if ((spin & 63) == 63) {
       if (*reinterpret_cast<volatile int*>(abort_flag) != 0) return false;
       unsigned long long now;
@@ -107,6 +112,9 @@ __device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, int* ab
       }
     }
   }
+}
+__device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, int* abort_flag) {
+  return try_wait(bar, parity) || wait_on(bar, parity, abort_flag);
 }
 // The whole warp waits and every lane gets the same answer.
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int* abort_flag) {
@@ -481,6 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     if (at < static_cast<int64_t>(p.B - 1) * p.bt_stride + p.cols) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(p.bt + at));
   }
   bool falls = false;                         // a bound below the one before it
+#pragma unroll 1
   for (int g = tid; g <= p.NG; g += kThreads) {
     const int start = p.group_start[g];
     falls |= g < p.NG && p.group_start[g + 1] < start;
@@ -488,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     if (g < min(p.NG, kSpGroupsNear)) s_bounds[kSpGroupsNear + 1 + g] = min(max(p.prefix_pages[g], 0), p.cols);
   }
   if (warp == 2 && lane == 0) {
+#pragma unroll 1
     for (uint32_t i = 0; i < 2 * NS; ++i) mbar_init(bars + 8 * i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull(i), 1);
@@ -514,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   const SpBounds bounds{p, n_groups, s_bounds, s_bounds + kSpGroupsNear + 1};
   SpItem mine{};
   int W = 0, my_cost = 0, my_at = 0, first_sum = 0;
+#pragma unroll 1
   for (int i0 = 0; i0 < n_items; i0 += kThreads) {
     const int i = i0 + tid;
     SpItem x{};
@@ -535,6 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   if (!idle) {
     if (my_cost > 0 && my_at <= x0 && x0 < my_at + my_cost) { *s_first = mine; s_plan[12] = tid; s_plan[13] = my_at; }
     int before = first_sum;
+#pragma unroll 1
     for (int i0 = kThreads; i0 < n_items && before <= x0; i0 += kThreads) {
       const int i = i0 + tid;
       SpItem x{};
@@ -552,6 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
   const uint32_t tmem = *tmem_slot;           // columns: S0 0, S1 128, O0 256, O1 384
 
   if (cta == 0 && warp >= 4) {                // these warps have nothing to do yet
+#pragma unroll 1
     for (int b = tid - 128; b < p.B; b += kThreads - 128) {
       const int g = p.sequences[b].group_at;  // the group's number so far
       const SpGroup gr = g >= 0 ? p.groups[g] : SpGroup{0, 0, 0, 0};
@@ -610,13 +623,16 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
         const uint32_t dst = q_buffer(qb), step = small ? 1024 : kPiece, bar = qfull(qb);
         if (r.spread == 32) {
           mbar_expect_tx(bar, NP * kPiece);
+#pragma unroll 1
           for (int piece = 0; piece < NP; ++piece)
             tma_load(dst + piece * step, &map_q, 0, (piece * p.HKV + r.head) * rows_head + r.row0, bar);
         } else {
           // eight rows at a time, eight or sixteen to a quarter of the 64
           const int boxes = (r.rows + 7) / 8;
           mbar_expect_tx(bar, NP * boxes * 1024);
+#pragma unroll 1
           for (int piece = 0; piece < NP; ++piece)
+#pragma unroll 1
             for (int i = 0; i < boxes; ++i)
               tma_load(dst + piece * step + i * (r.spread == 16 ? 1024 : 2048), &map_q8, 0,
                        (piece * p.HKV + r.head) * rows_head + r.row0 + 8 * i, bar);
@@ -625,9 +641,8 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       __syncwarp();
       return true;
     };
-    // q of a later run is asked for after the run's first tile, which need not wait until a q buffer is free
+    // q is asked for after the run's first tile, which need not wait until the pieces of q are there or a q buffer is free
     auto load = [&](const Run& r) -> bool {
-      if (listed == 1 && !load_q(r)) return false;
       const int32_t* row = p.bt + static_cast<int64_t>(r.table_row) * p.bt_stride;
       const int col0 = r.tok0 / kPage, cols = (r.end + kPage - 1) / kPage;         // cols <= p.cols
       auto page_at = [&](int col) {
@@ -666,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
           }
         }
         issued += n_pages;
-        if (t == 0 && listed > 1 && !load_q(r)) return false;
+        if (t == 0 && !load_q(r)) return false;
       }
       return true;
     };
@@ -699,14 +714,14 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       return true;
     };
     const int first_item = s_plan[12];
-    SpItem it = *s_first;
-    ok = runs_of(it, first_item < p.B);
+    SpItem it;
 #pragma unroll 1
-    for (int i0 = first_item + 1; ok && i0 < n_items && place < x1; i0 += 32) {
-      // 32 items, one to a lane; one that has tiles after the other
+    for (int i0 = first_item; ok && i0 < n_items && place < x1; i0 += i0 == first_item ? 1 : 32) {
+      // the first item by itself: it is known; then 32, one to a lane; one that has tiles after the other
       const int i = i0 + lane;
       SpItem x{};
-      if (i < n_items) x = sp_item(p, bounds, i, i < p.B ? p.seq_lens[i] : 0);
+      if (i0 == first_item) { if (lane == 0) x = *s_first; }
+      else if (i < n_items) x = sp_item(p, bounds, i, i < p.B ? p.seq_lens[i] : 0);
       uint32_t todo = __ballot_sync(0xffffffffu, x.tiles > 0 && x.units > 0);
 #pragma unroll 1
       while (todo && ok && place < x1) {
@@ -738,6 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       const uint32_t idesc = instr(0, p.fp8 == FFA_E4M3 ? 0 : 1, 0, r.spread == 32 ? 128 : 64);
       const uint64_t dq = desc(q_buffer(qb), 16);
       const uint32_t q_step = (small ? 1024 : kPiece) >> 4;
+#pragma unroll 1
       for (int t = 0; t < r.tiles; ++t, ++e) {
         const uint32_t s0 = pos % NS, s1 = (pos + 1) % NS, g = e & 1;
         if (!wait(full(s0), (pos / NS) & 1, aborted)) { ok = false; break; }
@@ -776,16 +792,19 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       const uint32_t idesc = instr(VBF16 ? 1 : 0, VBF16 ? 1 : 0, 1, r.spread == 32 ? 128 : 64);
       if (n_run >= 2 && !wait(ofree(o), ((n_run >> 1) - 1) & 1, aborted)) break;
       ++n_run;
+#pragma unroll 1
       for (int t = 0; t < r.tiles && ok; ++t, ++e) {
         const int valid = min(kSpTile, r.end - (r.tok0 + t * kSpTile)), pages = valid > kPage ? 2 : 1;
         const uint32_t g = e & 1;
         pos += nk;
+#pragma unroll 1
         for (int i = 0; i < pages && ok; ++i) {
           const uint32_t n = pos + i, v = s_ring + n % NS * kSlot;
           if (!wait(full(n % NS), (n / NS) & 1, aborted)) { ok = false; break; }
           const int here = valid - i * kPage;
           if (here < kPage && here % 16) {
             // tokens past the end of the sequence: whatever their V holds, 0 * V has to be 0
+#pragma unroll 1
             for (int x = lane; x < (16 - here % 16) * 16; x += 32) {
               const int row = here + x / 16, h = (x >> 3) & 1, ck = x & 7;
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n" ::"r"(v + h * 8192 + row * 128 + ck * 16), "r"(0) : "memory");
@@ -798,6 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
         fence_after();
         if (elect()) {
           const uint32_t a = tmem + 128 * g;
+#pragma unroll 1
           for (int i = 0; i < pages; ++i) {
             const uint64_t dv = desc(s_ring + (pos + i) % NS * kSlot, 8192);
             const int ks = min(4, (valid - i * kPage + 15) / 16);
