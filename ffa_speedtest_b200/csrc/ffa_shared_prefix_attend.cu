@@ -4,7 +4,8 @@
 //
 //   S[128 rows, 128 tokens] = sum over pieces of q, base and residual:  Qpiece . K^T    kind::f8f6f4, fp32 in TMEM
 //   P = 2^(S * row scale - m)                                                           one row per thread
-//   O[128 rows, 128 channels] += P . V                                                  kind::f16, P from TMEM
+//   O[128 rows, 128 channels] += P . V                                                  kind::f16, P from TMEM, in pieces
+//                                                                                       too where V is bfloat16
 //
 // K is used as it lies in the cache: q comes as e4m3 pieces (ffa_shared_prefix.cu), and the products of every piece with
 // the raw base and residual bytes accumulate into one fp32 tile.  That costs 4 (6) times the fp8 MMAs of one product,
@@ -226,6 +227,18 @@ __device__ __forceinline__ void tmem_st_16x128(uint32_t addr, const uint32_t (&r
       "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_16x128(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t (&r)[8], uint32_t addr) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
@@ -261,12 +274,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {       // NaN 
   asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// Weights as the MMA takes them, two tokens to a word.  float16: eleven bits.  bfloat16 has only eight, so there a weight is
+// two of them, the leading eight bits (cut off) and the rest, rounded to eight more: sixteen bits.  Up to 64 query rows the
+// rest has rows of the MMA to itself that were idle; with more the MMAs of P V are issued twice.  One piece would be faster,
+// by 38.3 to 39.0 us (8 samples of 32K), 40.1 to 41.6 (ragged prompts), 74.3 to 75.8 (16 private) and, with 128 rows, 260 to
+// 296 (64 samples of 128K); but its rounding is as large as that of a bfloat16 output, and larger than that of any other.
 template <bool BF16>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack16(float2 w) {
   uint32_t r;
-  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(w.y), "f"(w.x));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(w.y), "f"(w.x));
   return r;
+}
+__device__ __forceinline__ void two_pieces(float2 w, uint32_t& lead, uint32_t& rest) {
+  const uint32_t x = __float_as_uint(w.x), y = __float_as_uint(w.y);
+  lead = __byte_perm(x, y, 0x7632);
+  rest = pack16<true>(add2(w, make_float2(__uint_as_float((x & 0xffff0000u) ^ 0x80000000u), __uint_as_float((y & 0xffff0000u) ^ 0x80000000u))));
 }
 
 // What a softmax thread knows of a query row.
@@ -283,9 +306,12 @@ struct Row {
 // weights down to 2^-21 of it keep all eleven bits, and one below is off by at most 2^-32 of it.  With the largest at 2^0 the
 // weights of tokens 25 bits below one (an attention sink) were off by half, and l has them unrounded.  At 2^9 and 2^11, with
 // less room to rise before O is rescaled, 32 samples of 16K took 47.7 and 48.9 us, at 2^7 46.9, at 2^0 47.0.
+//
+// bfloat16 has the range.  There the largest weight is put at 2^0.3 and not at 1, whose second piece would be zero: a value
+// of infinity times it is NaN.
 template <bool VBF16>
 __device__ __forceinline__ float take_maximum(Row& row, float top, bool have_o, bool& lift) {
-  constexpr float kTop = VBF16 ? 0.f : 7.f, kMost = VBF16 ? 8.f : 15.f;
+  constexpr float kTop = VBF16 ? 0.3f : 7.f, kMost = VBF16 ? 8.f : 15.f;
   top = row.live ? top * row.scale : 0.f;     // the other rows' S is whatever lay in shared memory
   float up = 1.f;
   if (!(top <= row.m + kMost) || row.m == -INFINITY) {
@@ -298,22 +324,33 @@ __device__ __forceinline__ float take_maximum(Row& row, float top, bool have_o, 
   return up;
 }
 
-// S of a tile to P, in place; a row to a lane.  Tile begins at token `at`; bring_down(factor) rescales O.
+// S of a tile to P, in place; a row to a lane.  Tile begins at token `at`; bring_down(factor) rescales O.  16 tokens of P are
+// eight columns, with two pieces eight and eight.
 template <bool VBF16, typename F>
 __device__ __forceinline__ bool softmax_32(Row& row, uint32_t s_addr, int at, bool have_o, const F& bring_down) {
   const int lim = row.end - at;
   const bool cut = __any_sync(0xffffffffu, lim < kSpTile);
-  uint32_t x[128];
+  uint32_t x[32], y[32], z[32];               // three quarters of S at a time: the last two are read twice
   float top = -INFINITY;
   if (!cut) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_addr + 32 * c);
-    tmem_wait_ld();
     float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    auto tops_of = [&](const uint32_t* s) {
 #pragma unroll
-    for (int i = 0; i < 128; i += 8)
+      for (int i = 0; i < 32; i += 8)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tops[j] = max3(tops[j], __uint_as_float(x[i + j]), __uint_as_float(x[i + j + 4]));
+        for (int j = 0; j < 4; ++j) tops[j] = max3(tops[j], __uint_as_float(s[i + j]), __uint_as_float(s[i + j + 4]));
+    };
+    tmem_ld32(x, s_addr + 64);
+    tmem_ld32(y, s_addr + 96);
+    tmem_wait_ld();
+    tmem_ld32(z, s_addr);
+    tops_of(x);
+    tmem_ld32(x, s_addr + 32);
+    tops_of(y);
+    tmem_wait_ld();
+    tmem_ld32(y, s_addr + 64);
+    tops_of(z);
+    tops_of(x);
     top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
   } else {
 #pragma unroll 1
@@ -332,34 +369,56 @@ __device__ __forceinline__ bool softmax_32(Row& row, uint32_t s_addr, int at, bo
   const float neg = row.m == -INFINITY ? 0.f : -row.m;
   float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
   if (!cut) {
+    // quarter c of P, over what has been read of S
+    auto weights = [&](const uint32_t* s, int c) {
+      uint32_t w[32];
 #pragma unroll
-    for (int i = 0; i < 128; i += 4) {
-      float2 a = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), row.scale, neg);
-      float2 b = fma2(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), row.scale, neg);
-      a = make_float2(ex2(a.x), ex2(a.y));
-      b = make_float2(ex2(b.x), ex2(b.y));
-      sum = add2(sum, a);
-      sum1 = add2(sum1, b);
-      x[i / 2] = pack16<VBF16>(a.x, a.y);
-      x[i / 2 + 1] = pack16<VBF16>(b.x, b.y);
-    }
-    tmem_st32(s_addr, x);
-    tmem_st32(s_addr + 32, x + 32);
+      for (int i = 0; i < 32; i += 4) {
+        float2 a = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), row.scale, neg);
+        float2 b = fma2(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), row.scale, neg);
+        a = make_float2(ex2(a.x), ex2(a.y));
+        b = make_float2(ex2(b.x), ex2(b.y));
+        sum = add2(sum, a);
+        sum1 = add2(sum1, b);
+        if (VBF16) {
+          const int j = i / 16 * 16 + i % 16 / 2;
+          two_pieces(a, w[j], w[8 + j]);
+          two_pieces(b, w[j + 1], w[8 + j + 1]);
+        } else {
+          w[i / 2] = pack16<false>(a);
+          w[i / 2 + 1] = pack16<false>(b);
+        }
+      }
+      if (VBF16) tmem_st32(s_addr + 32 * c, w);
+      else tmem_st16(s_addr + 16 * c, w);
+    };
+    weights(z, 0);
+    tmem_ld32(z, s_addr + 96);
+    weights(x, 1);
+    tmem_wait_ld();
+    weights(y, 2);
+    weights(z, 3);
   } else {
-    // P of 32 tokens takes 16 columns, so it never reaches an S that is still to be read
+    // P of 32 tokens takes 16 or 32 columns, so it never reaches an S that is still to be read
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
       uint32_t y[32];
       tmem_ld32(y, s_addr + 32 * c);
       tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 32; i += 2) {
-        float2 a = fma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), row.scale, neg);
-        a = make_float2(32 * c + i < lim ? ex2(a.x) : 0.f, 32 * c + i + 1 < lim ? ex2(a.y) : 0.f);
-        sum = add2(sum, a);
-        y[i / 2] = pack16<VBF16>(a.x, a.y);
+      for (int i0 = 0; i0 < 32; i0 += 16) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float2 a = fma2(make_float2(__uint_as_float(y[i0 + i]), __uint_as_float(y[i0 + i + 1])), row.scale, neg);
+          a = make_float2(32 * c + i0 + i < lim ? ex2(a.x) : 0.f, 32 * c + i0 + i + 1 < lim ? ex2(a.y) : 0.f);
+          sum = add2(sum, a);
+          if (VBF16) two_pieces(a, w[i / 2], w[8 + i / 2]);
+          else y[(i0 + i) / 2] = pack16<false>(a);
+        }
+        if (VBF16) tmem_st16(s_addr + 32 * c + i0, w);
       }
-      tmem_st16(s_addr + 16 * c, y);
+      if (!VBF16) tmem_st16(s_addr + 16 * c, y);
     }
   }
   row.l = row.l * up + ((sum.x + sum.y) + (sum1.x + sum1.y));
@@ -368,7 +427,8 @@ __device__ __forceinline__ bool softmax_32(Row& row, uint32_t s_addr, int at, bo
 }
 
 // The same for up to 8 * H rows in the warp's first 16 TMEM lanes, four lanes of the warp to a row: lane i has columns
-// 8 * a + 2 * (i % 4), + 1 of rows i / 4 and i / 4 + 8.  A warp then works out 32 * H exponentials a lane, not 128.
+// 8 * a + 2 * (i % 4), + 1 of rows i / 4 and i / 4 + 8.  A warp then works out 32 * H exponentials a lane, not 128.  The second
+// piece of bfloat16 weights goes to the TMEM lanes 8 * H further on, and so does its part of O.
 template <int H, bool VBF16, typename F>
 __device__ __forceinline__ bool softmax_16(Row (&row)[2], uint32_t s_addr, int at, bool have_o, const F& bring_down) {
   const int lane = threadIdx.x & 31, col0 = 2 * (lane & 3);
@@ -395,29 +455,48 @@ __device__ __forceinline__ bool softmax_16(Row (&row)[2], uint32_t s_addr, int a
     up[h] = take_maximum<VBF16>(row[h], max3(top, z, z), have_o, lift);
   }
   if (__any_sync(0xffffffffu, lift)) {
-    const float a = __shfl_sync(0xffffffffu, up[0], (lane & 7) * 4), b = __shfl_sync(0xffffffffu, up[1], (lane & 7) * 4);
-    if (!bring_down(lane < 8 ? a : lane < 16 ? b : 1.f)) return false;
+    const float a = __shfl_sync(0xffffffffu, up[0], (lane & 7) * 4), b = __shfl_sync(0xffffffffu, up[H - 1], (lane & 7) * 4);
+    if (!bring_down(lane & 8 ? b : a)) return false;
   }
-  uint32_t w[32];
+  float neg[H];
+  float2 sum[H];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (h >= H) {
-#pragma unroll
-      for (int a = 0; a < 16; ++a) w[2 * a + h] = 0u;
-      continue;
-    }
-    const float neg = row[h].m == -INFINITY ? 0.f : -row[h].m;
-    float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int a = 0; a < 16; ++a) {
-      float2 v = fma2(make_float2(__uint_as_float(x[4 * a + 2 * h]), __uint_as_float(x[4 * a + 2 * h + 1])), row[h].scale, neg);
-      v = make_float2(ex2(v.x), ex2(v.y));
-      sum = add2(sum, v);
-      w[2 * a + h] = pack16<VBF16>(v.x, v.y);
-    }
-    row[h].l = row[h].l * up[h] + (sum.x + sum.y);
+  for (int h = 0; h < H; ++h) {
+    neg[h] = row[h].m == -INFINITY ? 0.f : -row[h].m;
+    sum[h] = make_float2(0.f, 0.f);
   }
-  tmem_st_16x128(s_addr, w);
+  auto weight = [&](const uint32_t* s, int h, int a) {
+    const int i = 4 * a + 2 * h;
+    float2 v = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), row[h].scale, neg[h]);
+    v = make_float2(ex2(v.x), ex2(v.y));
+    sum[h] = add2(sum[h], v);
+    return v;
+  };
+  if (H == 2 && VBF16) {
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {    // 64 tokens at a time
+      uint32_t w[16], rest[16];
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int a = 0; a < 8; ++a) two_pieces(weight(x, h, 8 * part + a), w[2 * a + h], rest[2 * a + h]);
+      tmem_st_16x128(s_addr + 32 * part, w);
+      tmem_st_16x128(s_addr + 32 * part + (16u << 16), rest);
+    }
+  } else {
+    uint32_t w[32];
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int a = 0; a < 16; ++a) {
+        if (VBF16) two_pieces(weight(x, h, a), w[2 * a], w[2 * a + 1]);
+        else w[2 * a + h] = pack16<false>(weight(x, h, a));
+        if (!VBF16 && H == 1) w[2 * a + 1] = 0u;
+      }
+    tmem_st_16x128(s_addr, w);
+  }
+#pragma unroll
+  for (int h = 0; h < H; ++h) row[h].l = row[h].l * up[h] + (sum[h].x + sum[h].y);
   tmem_wait_st();
   return true;
 }
@@ -575,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     }
   }
 
-  // The next run for a consumer warp, in order; false at the end (or when the CTA gave up).
+  // The next run for an MMA warp, in order; false at the end (or when the CTA gave up).
   uint32_t runs_read = 0;
   auto next_run = [&](Run& r) -> bool {
     const uint32_t i = runs_read % kRuns;
@@ -789,7 +868,8 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     bool ok = true;
     while (ok && next_run(r)) {
       const uint32_t o = n_run & 1, d = tmem + 256 + 128 * o;
-      const uint32_t idesc = instr(VBF16 ? 1 : 0, VBF16 ? 1 : 0, 1, r.spread == 32 ? 128 : 64);
+      const uint32_t type = VBF16 ? 1 : 0, idesc = instr(type, type, 1, r.spread == 32 || (VBF16 && r.spread == 16) ? 128 : 64);
+      const bool wide = VBF16 && r.spread == 32;
       if (n_run >= 2 && !wait(ofree(o), ((n_run >> 1) - 1) & 1, aborted)) break;
       ++n_run;
 #pragma unroll 1
@@ -823,7 +903,11 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
             const int ks = min(4, (valid - i * kPage + 15) / 16);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (k < ks) mma_16_tmem(d, a + 32 * i + 8 * k, dv + 128 * k, idesc, t > 0 || i + k > 0);
+              if (k < ks) {
+                const uint32_t p0 = a + (32 * i + 8 * k) * (wide ? 2 : 1);
+                mma_16_tmem(d, p0, dv + 128 * k, idesc, t > 0 || i + k > 0);
+                if (wide) mma_16_tmem(d, p0 + 8, dv + 128 * k, idesc, 1);
+              }
           }
           commit(sfree(g));
           for (int i = 0; i < pages; ++i) commit(empty((pos + i) % NS));
@@ -837,55 +921,84 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     const int quarter = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     uint32_t e = 0, n_run = 0;
-    // a finished run whose O is still to be written, a row to a lane
-    bool have_o = false, o_live = false;
-    int64_t o_part = 0;
-    int o_rows = 0, o_row = 0;
-    float o_m = 0.f, o_l = 0.f;
-    auto write_o = [&](uint32_t o) {
-      if (__any_sync(0xffffffffu, o_live)) {
-        float4* const dst = p.part_o + 32 * o_part + o_row;
+    // rows of a run in this quarter: lanes for them (a row to a lane with 32, else four lanes to each), first, number
+    auto rows_per = [&](int spread) { return spread ? spread : 8; };
+    auto rows_here = [&](int spread, int rows) { return spread || quarter == 0 ? min(rows_per(spread), rows - quarter * rows_per(spread)) : 0; };
+    // writes the O of the run before and gives the run back
+    auto write_o = [&]() {
+      const uint32_t n = n_run - 1;
+      const Run& done = runs[n % kRuns];
+      const int per = rows_per(done.spread), rows = done.rows, here = rows_here(done.spread, rows), first = quarter * per;
+      const uint32_t o_addr = lanes + 256 + 128 * (n & 1);
+      if (here > 0) {
+        if (per == 32) {
+          float4* const dst = p.part_o + 32 * done.part + first + lane;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          tmem_ld32(x, lanes + 256 + 128 * o + 32 * c);
-          tmem_wait_ld();
-          if (o_live)
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            tmem_ld32(x, o_addr + 32 * c);
+            tmem_wait_ld();
+            if (lane < here)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[static_cast<int64_t>(8 * c + i) * o_rows] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]),
+              for (int i = 0; i < 8; ++i)
+                dst[static_cast<int64_t>(8 * c + i) * rows] = make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]),
                                                                           __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3]));
+          }
+        } else {
+          // four lanes to a row, two channels of every eight to a lane; with bfloat16 weights O of the second pieces is added
+          float2* const dst = reinterpret_cast<float2*>(p.part_o + 32 * done.part + first + (lane >> 2)) + (lane & 1);
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t x[8], y[8];
+            tmem_ld_16x256(x, o_addr + 16 * c);
+            if (VBF16 && per == 16) tmem_ld_16x256(y, o_addr + 16 * c + (16u << 16));
+            tmem_wait_ld();
+            if (VBF16) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(per == 16 ? y[i] : x[i ^ 2]));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i += 2)
+              if ((lane >> 2) + 4 * (i & 2) < here)
+                dst[static_cast<int64_t>(4 * c + 2 * (i >> 2) + ((lane >> 1) & 1)) * 2 * rows + 8 * (i & 2)] =
+                    make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          }
         }
-        if (o_live) p.part_ml[o_part + o_row] = make_float2(o_m, o_l);
       }
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ofree(o));
+      if (lane == 0) {
+        mbar_arrive(ofree(n & 1));
+        mbar_arrive(runempty(n % kRuns));
+      }
     };
-    Run r;
     bool ok = true;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    while (ok && next_run(r)) {
-      // rows of this quarter: first, number; a row to a lane (32), or up to 8 or 16 rows with four lanes to each
-      const int per = r.spread ? r.spread : 8, first_row = quarter * per;
-      const int here = r.spread || quarter == 0 ? min(per, r.rows - first_row) : 0;
-      const bool any_live = here > 0;
+    for (;;) {
+      if (!wait(runfull(n_run % kRuns), (n_run / kRuns) & 1, aborted)) break;
+      const Run& r = runs[n_run % kRuns];
+      const bool more = r.tiles > 0;
+      if (!more && n_run == 0) break;
+      const int per = rows_per(r.spread);
+      const bool any_live = rows_here(r.spread, r.rows) > 0;
       Row row[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int j = per == 32 ? lane : (lane >> 2) + 8 * h;
         row[h] = Row{};
-        row[h].live = j < here && (h == 0 || per == 16);
+        row[h].live = j < rows_here(r.spread, r.rows) && (h == 0 || per == 16);
         row[h].end = r.end;
         if (row[h].live) {
-          row[h].scale = p.q_scale[static_cast<int64_t>(r.head) * p.B * p.G + r.row0 + first_row + j];
-          row[h].end = min(r.end, p.seq_lens[(r.row0 + first_row + j) / p.G]);
+          const int at = r.row0 + quarter * per + j;
+          row[h].scale = p.q_scale[static_cast<int64_t>(r.head) * p.B * p.G + at];
+          row[h].end = min(r.end, p.seq_lens[at / p.G]);
         }
       }
-      const uint32_t o_addr = lanes + 256 + 128 * (n_run & 1);
-      for (int t = 0; t < r.tiles; ++t, ++e) {
+      // after the last run once more, for its O
+#pragma unroll 1
+      for (int t = 0; t < max(r.tiles, 1); ++t, ++e) {
         const uint32_t g = e & 1, s_addr = lanes + 128 * g;
-        if (!wait(sfull(g), (e >> 1) & 1, aborted)) { ok = false; break; }
+        if (more && !wait(sfull(g), (e >> 1) & 1, aborted)) { ok = false; break; }
         fence_after();
         // PV of the step before is done: O may be brought down
         bool waited = false;
@@ -898,6 +1011,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
         // O is rescaled by a factor per row, a row to a lane
         auto bring_down = [&](float up) -> bool {
           if (!pv_done()) return false;
+          const uint32_t o_addr = lanes + 256 + 128 * (n_run & 1);
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
             uint32_t y[16];
@@ -918,35 +1032,24 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
         if (!ok || !pv_done()) { ok = false; break; }
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pfull(g));
-        if (t == 0 && have_o) {
-          write_o((n_run - 1) & 1);
-          have_o = false;
-        }
+        if (more && lane == 0) mbar_arrive(pfull(g));
+        if (t == 0 && n_run > 0) write_o();
       }
-      if (!ok) break;
-      have_o = true;
-      o_live = lane < here;
-      o_part = r.part;
-      o_rows = r.rows;
-      o_row = first_row + lane;
-      if (per == 32) {
-        o_m = row[0].m;
-        o_l = row[0].l;
-      } else {
+      if (!ok || !more) break;
+      // maxima and sums are written now, O when the next run has begun
+      if (per != 32) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           row[h].l += __shfl_xor_sync(0xffffffffu, row[h].l, 1);
           row[h].l += __shfl_xor_sync(0xffffffffu, row[h].l, 2);
-          const float m = __shfl_sync(0xffffffffu, row[h].m, (lane & 7) * 4), l = __shfl_sync(0xffffffffu, row[h].l, (lane & 7) * 4);
-          if (lane >> 3 == h) { o_m = m; o_l = l; }
         }
       }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = per == 32 ? lane : (lane >> 2) + 8 * h;
+        if (row[h].live && (per == 32 || (lane & 3) == 0)) p.part_ml[r.part + quarter * per + j] = make_float2(row[h].m, row[h].l);
+      }
       ++n_run;
-    }
-    if (ok && have_o && wait(sfree((e - 1) & 1), ((e - 1) >> 1) & 1, aborted)) {
-      fence_after();
-      write_o((n_run - 1) & 1);
     }
   }
 
