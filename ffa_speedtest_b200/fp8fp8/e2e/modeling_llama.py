@@ -148,10 +148,8 @@ class LlamaAttention(nn.Module):
             past_key_values.update(k, v, self.layer_idx)
             if T == 1:
                 attn = past_key_values.decode(q.contiguous(), self.layer_idx, settings.get("scale")).view(B, 1, self.num_heads, self.head_dim)
-            elif past_key_values.get_seq_length() == T:
-                attn = _dense_attention(q, k, v, causal=True)                     # prefill from empty sequences
             else:
-                raise RuntimeError("a SharedPrefixFP8Fp8Cache serves prefill from empty sequences and single-token steps")
+                attn = _dense_attention(q, k, v, causal=True)                     # prefill from empty sequences
         elif isinstance(past_key_values, PagedFP8Fp8Cache):
             ffa_step = T == 1 and use_ffa_decode and in_pattern
             if ffa_step and settings.get("fused_append", True) and past_key_values.use_fp8_residual:
@@ -220,12 +218,28 @@ class LlamaForCausalLM(nn.Module):
             raise ValueError(f"position {start + count} exceeds max_position_embeddings {self._rope[0].shape[0]}")
         return self._rope[0][start:start + count], self._rope[1][start:start + count]
 
+    def _check_shared(self, cache: SharedPrefixFP8Fp8Cache, B: int, T: int) -> None:
+        """Refuse a call before it takes room in the cache: afterwards its sequences would hold tokens that no layer wrote."""
+        cfg, held = self.config, cache.get_seq_length()
+        if (cache.num_kv_heads, cache.head_dim) != (cfg.num_key_value_heads, cfg.head_dim) or cache.num_layers < cfg.num_hidden_layers:
+            raise ValueError(f"the cache is for {cache.num_layers} layers of {cache.num_kv_heads} kv-heads of {cache.head_dim}, the model has "
+                             f"{cfg.num_hidden_layers} of {cfg.num_key_value_heads} of {cfg.head_dim}")
+        if cfg.num_attention_heads > 8 * cfg.num_key_value_heads:
+            raise ValueError(f"this build supports GQA group sizes up to 8, got {cfg.num_attention_heads // cfg.num_key_value_heads}")
+        if B != len(cache.active):
+            raise ValueError(f"{len(cache.active)} sequences are active, input_ids has {B} rows")
+        if T > 1 and held > 0:
+            raise RuntimeError("a SharedPrefixFP8Fp8Cache serves prefill from empty sequences and single-token steps")
+        if held + T > cfg.max_position_embeddings:
+            raise ValueError(f"position {held + T} exceeds max_position_embeddings {cfg.max_position_embeddings}")
+
     @torch.no_grad()
     def forward(self, input_ids: torch.Tensor, past_key_values=None, use_cache: bool = False) -> torch.Tensor:
         cache = past_key_values if use_cache else None
         x = self.embed_tokens(input_ids)
         T = input_ids.shape[1]
         if isinstance(cache, SharedPrefixFP8Fp8Cache):
+            self._check_shared(cache, input_ids.shape[0], T)
             cache.extend(T)
             cos, sin = self._rope_rows(0, cache.get_seq_length(), x.dtype, x.device)
             at = cache.positions()

@@ -71,6 +71,11 @@ class SharedPrefixFP8Fp8Cache:
         self._new = 0
         self._group()
 
+    @property
+    def active(self) -> tuple[int, ...]:
+        """The sequences that ``activate`` named."""
+        return tuple(self._seqs)
+
     def _alone(self, s: int) -> None:
         """The sequence begins a line of its own."""
         self._line[s], self._shared[s], self._held[s] = self._next_line, self.max_seq_len // PAGE, 0

@@ -199,6 +199,38 @@ def test_refusals():
         model(torch.zeros(1, 2, dtype=torch.long, device="cuda"), past_key_values=cache, use_cache=True)
 
 
+def test_a_refused_model_call_leaves_the_cache_as_it_was():
+    cfg, model = build()
+    make = lambda n=2, kv=2, layers=2: SharedPrefixFP8Fp8Cache(n, kv, 1024, num_layers=layers)
+    ids = lambda b, t: torch.ones(b, t, dtype=torch.long, device="cuda")
+    cache = make()
+    cache.activate([0])
+    model(ids(1, 511), past_key_values=cache, use_cache=True)              # one position is left of the model's 512
+    model(ids(1, 1), past_key_values=cache, use_cache=True)
+    other = make()
+    other.activate([0, 1])
+
+    def refused(c, tokens, error, match):
+        before = [c.table.seq_lens.clone(), c.table.block_table.clone(), c.table.refcount.clone(), *(x.clone() for x in c.table.pools)]
+        lengths = list(c.lengths)
+        with pytest.raises(error, match=match):
+            model(tokens, past_key_values=c, use_cache=True)
+        after = [c.table.seq_lens, c.table.block_table, c.table.refcount, *c.table.pools]
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, after)) and c.lengths == lengths
+
+    refused(cache, ids(1, 1), ValueError, "max_position")
+    refused(cache, ids(1, 3), RuntimeError, "prefill from empty")
+    refused(other, ids(2, 513), ValueError, "max_position")
+    refused(other, ids(1, 4), ValueError, "2 sequences are active")
+    refused(other, ids(3, 1), ValueError, "2 sequences are active")
+    refused(make(), ids(1, 1), ValueError, "0 sequences are active")
+    for wrong in (make(kv=1), make(layers=1)):
+        wrong.activate([0])
+        refused(wrong, ids(1, 1), ValueError, "the cache is for")
+    model(ids(2, 5), past_key_values=other, use_cache=True)
+    other.check()
+
+
 def test_driver_with_samples():
     r = subprocess.run([sys.executable, "-m", "ffa_speedtest_b200.fp8fp8.e2e.bench_llama_fp8fp8", "--context", "300", "--samples", "3",
                         "--decode-steps", "70", "--batch", "2", "--iters", "2", "--warmup", "1", "--json"], cwd=ROOT, capture_output=True,
