@@ -17,11 +17,43 @@ from __future__ import annotations
 
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from ...pages import PageTable, append_ragged_fp8fp8
 from ..attn_kernel.attn_kernel_shared_prefix_fp8fp8 import SharedPrefixWorkspace, attn_forward_decode_shared_prefix_fp8fp8
 from .fp8fp8_cache import PAGE, resolve_fp8_dtype
+
+
+def _stretches(common: np.ndarray) -> tuple[list[int], list[int]]:
+    """Cut a batch into groups.  ``common[i]``: pages that sequences i and i + 1 share.  The first sequence of every group
+    and the batch's end, and the pages that all of a group have in common: the cut that saves the most reading of pages, a
+    group of n with m pages in common saving (n - 1) * m.  One group for each stretch that shares the same number
+    throughout (samples of one prompt); a stretch of forks of forks is cut by dynamic programming."""
+    n = len(common) + 1
+    cuts = [0, *(np.flatnonzero(common == 0) + 1).tolist(), n]
+    start, pages = [], []
+    for a, b in zip(cuts[:-1], cuts[1:]):
+        c = common[a:b - 1]
+        if b - a == 1 or (c == c[0]).all():
+            start.append(a)
+            pages.append(int(c[0]) if b - a > 1 else 0)
+            continue
+        best, first = np.zeros(b - a + 1, dtype=np.int64), np.zeros(b - a + 1, dtype=np.int64)
+        for j in range(1, b - a + 1):                         # best cut of the first j; its last group is first[j] .. j - 1
+            least = np.minimum.accumulate(np.append(c[:j - 1], 0)[::-1][1:])[::-1] if j > 1 else c[:0]
+            saved = best[:j] + np.append(least * np.arange(j - 1, 0, -1), 0)
+            first[j] = saved.argmax()
+            best[j] = saved[first[j]]
+        groups = []
+        while b > a:
+            i = a + int(first[b - a])
+            groups.append((i, int(common[i:b - 1].min()) if b - i > 1 else 0))
+            b = i
+        for i, m in reversed(groups):
+            start.append(i)
+            pages.append(m)
+    return [*start, n], pages
 
 
 class SharedPrefixFP8Fp8Cache:
@@ -44,11 +76,10 @@ class SharedPrefixFP8Fp8Cache:
                                pools=[*self.key_base, *self.key_residual, *self.value])
         self.device = self.table.device
         self.lengths = [0] * max_seqs
-        # of every sequence: the prompt that its first pages come from, and how many of them are that prompt's
-        self._line = list(range(max_seqs))
-        self._shared = [self.max_seq_len // PAGE] * max_seqs
-        self._held = [0] * max_seqs               # pages of it that another sequence of that prompt may count on
-        self._next_line = max_seqs
+        # what is in every page of every sequence: equal numbers in a column are one page, a page gets a new number when
+        # it is written to
+        self._contents = np.full((max_seqs, pages_per_seq), -1, dtype=np.int64)
+        self._next_content = 0
         self._seqs: list[int] = []
         self._new = 0
         self._workspace: Optional[SharedPrefixWorkspace] = None
@@ -76,19 +107,18 @@ class SharedPrefixFP8Fp8Cache:
         """The sequences that ``activate`` named."""
         return tuple(self._seqs)
 
-    def _alone(self, s: int) -> None:
-        """The sequence begins a line of its own."""
-        self._line[s], self._shared[s], self._held[s] = self._next_line, self.max_seq_len // PAGE, 0
-        self._next_line += 1
+    def _written(self, s: int, first: int, end: int) -> None:
+        """Columns first .. end - 1 of the sequence get contents of their own."""
+        self._contents[s, first:end] = np.arange(self._next_content, self._next_content + max(0, end - first))
+        self._next_content += max(0, end - first)
 
     def _group(self) -> None:
-        """Stretches of the batch whose sequences come from one prompt, and the pages they have in common."""
-        start, pages = [0], []
-        for i in range(1, len(self._seqs) + 1):
-            if i == len(self._seqs) or self._line[self._seqs[i]] != self._line[self._seqs[i - 1]]:
-                members = self._seqs[start[-1]:i]
-                pages.append(min(min(self._shared[s], self.lengths[s] // PAGE) for s in members) if len(members) > 1 else 0)
-                start.append(i)
+        """Stretches of the batch whose sequences have their first full pages in common, and how many."""
+        lens = np.array([self.lengths[s] for s in self._seqs], dtype=np.int64) // PAGE
+        cols = max(1, int(lens.max()))
+        rows = self._contents[self._seqs, :cols]
+        same = (rows[1:] == rows[:-1]) & (np.arange(cols) < np.minimum(lens[1:], lens[:-1])[:, None])
+        start, pages = _stretches(np.where(same.all(1), cols, same.argmin(1)))      # the first page that is not the next one's too
         self._group_start = torch.tensor(start, dtype=torch.int32, device=self.device)
         self._prefix_pages = torch.tensor(pages, dtype=torch.int32, device=self.device)
 
@@ -101,12 +131,7 @@ class SharedPrefixFP8Fp8Cache:
             raise ValueError("the children must be empty: free them first")
         self.table.fork(parents, children)
         for p, c in zip(parents, children):
-            self.lengths[c], pages = self.lengths[p], min(self._shared[p], self.lengths[p] // PAGE)
-            if pages == 0:
-                self._alone(c)
-                continue
-            self._line[c], self._shared[c], self._held[c] = self._line[p], pages, pages
-            self._held[p] = max(self._held[p], pages)
+            self.lengths[c], self._contents[c] = self.lengths[p], self._contents[p]
         if self._seqs:
             self._group()
 
@@ -118,9 +143,13 @@ class SharedPrefixFP8Fp8Cache:
         self.table.truncate(seqs, new_lens)
         for s, n in zip(seqs, new_lens):
             if n < self.lengths[s]:
+                full, held = n // PAGE, -(-n // PAGE)
+                # cut back into pages that others hold too it goes on by itself: kept with them, it would hold down what
+                # all of them read once
+                if full < self.lengths[s] // PAGE and np.count_nonzero(self._contents[:, full] == self._contents[s, full]) > 1:
+                    self._written(s, 0, held)
+                self._contents[s, held:] = -1
                 self.lengths[s] = n
-                if n // PAGE < self._held[s]:         # its next pages will not be those that the others have
-                    self._alone(s)
         self._new = 0
         if self._seqs:
             self._group()
@@ -142,8 +171,9 @@ class SharedPrefixFP8Fp8Cache:
             self.table.check()
         except RuntimeError:
             self.lengths = self.table.seq_lens.tolist()
-            for s in range(len(self.lengths)):        # forks since then may share less than was written down
-                self._alone(s)
+            for s, n in enumerate(self.lengths):      # forks since then may share less than was written down
+                self._contents[s] = -1
+                self._written(s, 0, -(-n // PAGE))
             self._new = 0
             if self._seqs:
                 self._group()
@@ -165,6 +195,7 @@ class SharedPrefixFP8Fp8Cache:
         self.table.extend(self._rows, n_new)
         self._new = n_new
         for s in self._seqs:
+            self._written(s, self.lengths[s] // PAGE, -(-(self.lengths[s] + n_new) // PAGE))
             self.lengths[s] += n_new
         self._bt, self._lens = self.table.block_table[at], self.table.seq_lens[at]
         self._counts = self._lens - self._positions   # 0 where there were no pages: nothing is written then

@@ -156,6 +156,73 @@ def test_groups_through_forks_and_rejected_drafts():
     cache.check()
 
 
+def test_forks_of_a_grown_sample_share_what_it_wrote():
+    cache = SharedPrefixFP8Fp8Cache(8, 2, 768, num_layers=1)
+    pages = lambda: (cache._group_start.tolist(), cache._prefix_pages.tolist())
+    cache.activate([0])
+    cache.extend(200)
+    cache.fork([0, 0], [1, 2])
+    cache.activate([1])
+    cache.extend(500)                                       # the sample is 700 tokens long, 200 of them the prompt's
+    cache.fork([1, 1], [3, 4])
+    cache.activate([1, 3, 4])
+    assert pages() == ([0, 3], [10])
+    cache.activate([1, 3, 4, 0, 2])
+    assert pages() == ([0, 3, 5], [10, 3])
+    cache.activate([1, 0, 3])                               # not side by side: the prompt is what they have in common
+    assert pages() == ([0, 3], [3])
+    cache.free([0, 2])                                      # the prompt's end changes nothing for them
+    cache.activate([1, 3, 4])
+    cache.extend(60)
+    cache.fork([3], [5])
+    cache.activate([1, 3, 5, 4])
+    assert pages() == ([0, 4], [10])
+    cache.activate([3, 5, 4])
+    cache.extend(8)                                         # to the last token that a sequence can hold
+    assert pages() == ([0, 3], [10])
+    cache.activate([3, 5])
+    assert pages() == ([0, 2], [11])
+    cache.check()
+
+
+def test_forks_of_grown_samples_track_the_dense_model():
+    cfg, model = build()
+    g = torch.Generator().manual_seed(3)
+    draw = lambda n: torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist()
+    cache = SharedPrefixFP8Fp8Cache(8, 2, 512, num_layers=2, fp8_dtype=torch.float8_e4m3fn)
+    text = {0: draw(140)}
+    cache.activate([0])
+    model(torch.tensor([text[0]], device="cuda"), past_key_values=cache, use_cache=True)
+
+    def steps(seqs, n):
+        cache.activate(seqs)
+        for _ in range(n):
+            new = draw(len(seqs))
+            for s, x in zip(seqs, new):
+                text[s].append(x)
+            logits = model(torch.tensor(new, device="cuda")[:, None], past_key_values=cache, use_cache=True)[:, -1]
+        close(logits, dense_logits(model, cfg, [text[s] for s in seqs]))
+
+    def fork(parents, children):
+        cache.fork(parents, children)
+        for p, c in zip(parents, children):
+            text[c] = list(text[p])
+
+    fork([0, 0], [1, 2])
+    steps([1, 2], 70)
+    fork([1, 2, 1], [3, 4, 5])
+    steps([1, 3, 5, 0, 2, 4], 3)
+    assert (cache._group_start.tolist(), cache._prefix_pages.tolist()) == ([0, 6], [2])
+    steps([1, 3, 5, 2, 4], 2)
+    assert (cache._group_start.tolist(), cache._prefix_pages.tolist()) == ([0, 3, 5], [3, 3])
+    steps([2, 1, 4, 3, 5], 66)                              # out of order
+    cache.truncate([3, 4], [205, 150])
+    del text[3][205:], text[4][150:]
+    fork([3], [6])
+    steps([6, 3, 1, 5, 4, 2], 61)
+    cache.check()
+
+
 def test_decode_needs_an_extend_after_the_pages_changed():
     cache = SharedPrefixFP8Fp8Cache(4, 2, 256, num_layers=1)
     q, k = torch.zeros(1, 1, 4, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16, device="cuda")
