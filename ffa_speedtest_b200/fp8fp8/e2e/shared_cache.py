@@ -165,15 +165,18 @@ class SharedPrefixFP8Fp8Cache:
         self._new = 0
 
     def check(self) -> None:
-        """Raise if a call since the last check ran out of pages (waits for the device).  The lengths are then those on
-        the device, and no sequence counts as another's sample until it is forked anew."""
+        """Raise if a call since the last check ran out of pages (waits for the device).  Lengths, and which pages sequences
+        share, are then taken from the device, and work goes on from there; what model calls returned since the one that
+        ran out is not to be used."""
         try:
             self.table.check()
         except RuntimeError:
             self.lengths = self.table.seq_lens.tolist()
-            for s, n in enumerate(self.lengths):      # forks since then may share less than was written down
-                self._contents[s] = -1
-                self._written(s, 0, -(-n // PAGE))
+            # a page's number says what is in it; the numbers of pages that are written to from here on are others
+            rows = self.table.block_table.cpu().numpy().astype(np.int64)
+            held = np.arange(rows.shape[1]) < -(-np.array(self.lengths)[:, None] // PAGE)
+            self._contents = np.where(held & (rows >= 0), rows + self._next_content, -1)
+            self._next_content += self.table.n_pages
             self._new = 0
             if self._seqs:
                 self._group()

@@ -125,6 +125,59 @@ def test_without_pages_nothing_is_written_and_work_goes_on():
         close(logits, dense_logits(model, cfg, [text[1], text[2]]))
 
 
+def test_sharing_goes_on_after_running_out_of_pages():
+    cfg, model = build()
+    g = torch.Generator().manual_seed(6)
+    draw = lambda n: torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist()
+    cache = SharedPrefixFP8Fp8Cache(6, 2, 512, num_layers=2, n_pages=9, fp8_dtype=torch.float8_e4m3fn)
+    pages = lambda: (cache._group_start.tolist(), cache._prefix_pages.tolist())
+    text = {0: draw(150), 5: draw(60)}
+    for s in (0, 5):
+        cache.activate([s])
+        model(torch.tensor([text[s]], device="cuda"), past_key_values=cache, use_cache=True)
+    cache.fork([0] * 3, [1, 2, 3])                          # four pages are held
+    for s in (1, 2, 3):
+        text[s] = list(text[0])
+
+    def step(seqs):
+        new = draw(len(seqs))
+        logits = model(torch.tensor(new, device="cuda")[:, None], past_key_values=cache, use_cache=True)[:, -1]
+        for s, x in zip(seqs, new):
+            text[s].append(x)
+        return logits
+
+    seqs = [1, 2, 3, 5]
+    cache.activate(seqs)
+    for _ in range(4):                                      # three open pages are copied: two are left
+        logits = step(seqs)
+    close(logits, dense_logits(model, cfg, [text[s] for s in seqs]))
+    for _ in range(39):                                     # one goes to sequence 5, and at 192 tokens the others need three
+        step(seqs)
+    cache.fork([2], [4])                                    # forked before anyone has noticed
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache.check()
+    assert cache.lengths == cache.table.seq_lens.tolist()
+    for s in (*seqs, 4):
+        text[s] = text[2 if s == 4 else s][:cache.lengths[s]]
+    assert [cache.lengths[s] for s in (1, 2, 3, 4, 5)] == [192] * 4 + [102]
+    cache.activate([1, 2, 4, 3, 5])
+    assert pages() == ([0, 4, 5], [2, 0])                   # the prompt is read once still
+    cache.free([0])
+    cache.activate([1, 2, 4])
+    assert pages() == ([0, 3], [2])
+    step([1, 2, 4])
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache.check()                                       # three are needed, two are free
+    for s in (1, 2, 4):
+        del text[s][-1:]
+    cache.activate([2, 4])
+    assert pages() == ([0, 2], [3])
+    cache.free([1, 5])
+    logits = step([2, 4])
+    cache.check()
+    close(logits, dense_logits(model, cfg, [text[s] for s in (2, 4)]))
+
+
 def test_groups_through_forks_and_rejected_drafts():
     cache = SharedPrefixFP8Fp8Cache(6, 2, 1024, num_layers=1)
     pages = lambda: (cache._group_start.tolist(), cache._prefix_pages.tolist())
