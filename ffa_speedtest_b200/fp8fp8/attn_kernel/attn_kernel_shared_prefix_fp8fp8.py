@@ -27,6 +27,7 @@ class SharedPrefixWorkspace:
             raise ValueError(f"no workspace for B={B}, HQ={HQ}, HKV={HKV}: B must be 1 to 4096, HQ a multiple of HKV")
         self.scratch = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.scratch[:512].zero_()
+        self.status_word = self.scratch[256:260].view(torch.int32)
         self.o = torch.empty((self.B, self.HQ, 128), dtype=dtype, device=self.device)
 
     def matches(self, B: int, HQ: int, HKV: int, device, dtype) -> bool:
@@ -35,7 +36,7 @@ class SharedPrefixWorkspace:
     def status(self) -> int:
         """Device status word (synchronises): 0 = ok, 1 = a bounded wait inside a kernel gave up (the affected
         outputs are NaN)."""
-        return int(self.scratch[256:260].view(torch.int32).item())
+        return int(self.status_word.item())
 
 
 def allocate_shared_prefix_workspace(q: torch.Tensor, v: torch.Tensor) -> SharedPrefixWorkspace:

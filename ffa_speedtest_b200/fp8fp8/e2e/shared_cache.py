@@ -83,6 +83,7 @@ class SharedPrefixFP8Fp8Cache:
         self._seqs: list[int] = []
         self._new = 0
         self._workspace: Optional[SharedPrefixWorkspace] = None
+        self._gave_up = torch.zeros(1, dtype=torch.int32, device=self.device)         # of workspaces before the present one
 
     # ---- sequences ---------------------------------------------------------------------------------------
     def _numbers(self, seqs: Sequence[int]) -> list[int]:
@@ -167,7 +168,7 @@ class SharedPrefixFP8Fp8Cache:
     def check(self) -> None:
         """Raise if a call since the last check ran out of pages (waits for the device).  Lengths, and which pages sequences
         share, are then taken from the device, and work goes on from there; what model calls returned since the one that
-        ran out is not to be used."""
+        ran out is not to be used.  Raises too if a bounded wait inside the attention gave up: outputs are NaN then."""
         try:
             self.table.check()
         except RuntimeError:
@@ -181,6 +182,12 @@ class SharedPrefixFP8Fp8Cache:
             if self._seqs:
                 self._group()
             raise
+        if self._workspace is not None:
+            self._gave_up |= self._workspace.status_word
+            self._workspace.status_word.zero_()
+        if int(self._gave_up.item()):
+            self._gave_up.zero_()
+            raise RuntimeError("shared-prefix decode: a wait inside a kernel gave up, outputs since the last check may be NaN")
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         """Tokens of the longest active sequence."""
@@ -225,6 +232,8 @@ class SharedPrefixFP8Fp8Cache:
         self._extended()
         ws = self._workspace
         if ws is None or not ws.matches(q.shape[0], q.shape[2], self.num_kv_heads, q.device, q.dtype):
+            if ws is not None:
+                self._gave_up |= ws.status_word
             ws = self._workspace = SharedPrefixWorkspace(q.shape[0], q.shape[2], self.num_kv_heads, q.device, q.dtype)
         return attn_forward_decode_shared_prefix_fp8fp8(
             q, self.key_base[layer_idx], self.value[layer_idx], k_residual=self.key_residual[layer_idx], block_table=self._bt,

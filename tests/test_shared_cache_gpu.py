@@ -178,6 +178,31 @@ def test_sharing_goes_on_after_running_out_of_pages():
     close(logits, dense_logits(model, cfg, [text[s] for s in (2, 4)]))
 
 
+def test_check_reports_an_attention_that_gave_up():
+    """The word is set here by hand: no wait in the kernel depends on anything that a caller could hold back."""
+    cache = SharedPrefixFP8Fp8Cache(4, 2, 256, num_layers=1)
+    zeros = lambda b, h: torch.zeros(b, 1, h, 128, dtype=torch.bfloat16, device="cuda")
+
+    def step(seqs):
+        cache.activate(seqs)
+        cache.extend(1)
+        cache.update(zeros(len(seqs), 2), zeros(len(seqs), 2), 0)
+        cache.decode(zeros(len(seqs), 4), 0)
+
+    step([0, 1])
+    cache.check()
+    cache._workspace.status_word.fill_(1)
+    with pytest.raises(RuntimeError, match="gave up"):
+        cache.check()
+    cache.check()                                           # reported once
+    cache._workspace.status_word.fill_(1)
+    step([2])                                               # another workspace in the meantime
+    assert cache._workspace.status() == 0
+    with pytest.raises(RuntimeError, match="gave up"):
+        cache.check()
+    cache.check()
+
+
 def test_groups_through_forks_and_rejected_drafts():
     cache = SharedPrefixFP8Fp8Cache(6, 2, 1024, num_layers=1)
     pages = lambda: (cache._group_start.tolist(), cache._prefix_pages.tolist())
