@@ -648,7 +648,8 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       const int g = p.sequences[b].group_at;  // the group's number so far
       const SpGroup gr = g >= 0 ? p.groups[g] : SpGroup{0, 0, 0, 0};
       p.sequences[b].group_at = gr.at;
-      p.sequences[b].group_tiles = gr.tiles;
+      // one that holds nothing has no partials, whatever its q is (the padding of a batch)
+      p.sequences[b].group_tiles = p.seq_lens[b] > 0 ? gr.tiles : 0;
       p.sequences[b].group_first = gr.first;
       p.sequences[b].group_rows = gr.rows;
     }

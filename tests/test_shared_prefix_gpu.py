@@ -161,6 +161,24 @@ def test_lengths_of_zero_one_and_inside_the_prefix():
     assert bool((b.call() == 0).all())
 
 
+@pytest.mark.parametrize("sizes,prefix", [([3, 1], [2, 0]), ([40, 2], [3, 1])])
+def test_padding_that_holds_nothing_gives_zeros_whatever_its_q(sizes, prefix):
+    b = Batch(sizes, prefix, [20], 8, 2, seed=18)
+    empty = [0, 2, b.B - 1]
+    lens = [0 if i in empty else n for i, n in enumerate(b.lens)]
+    b.seq_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    b.seq_lens[0] = -5                                       # below zero is as good as zero
+    b.q[empty] = 0
+    want = b.call().clone()
+    b.check(want, lens=lens)
+    for bad in (math.nan, math.inf):
+        b.q[empty] = bad
+        part = torch.full((b.B, 8, 129), 7.0, device="cuda")
+        got = b.call(partial_out=part)
+        assert torch.equal(got, want)
+        assert bool((part[empty, :, :128] == 0).all()) and bool((part[empty, :, 128] == -math.inf).all())
+
+
 def test_garbage_outside_the_sequences():
     """NaN and infinities in the unused rows of pages, in unused pages and in unused table entries."""
     b = Batch([3, 2], [2, 0], [1, 65, 100], 8, 2, seed=6, spare=9)
