@@ -196,6 +196,7 @@ class SharedPrefixFP8Fp8Cache:
     # ---- a model call --------------------------------------------------------------------------------------
     def extend(self, n_new: int) -> None:
         """Room for ``n_new`` more tokens of every active sequence; once per model call, before its layers."""
+        self._not_captured()
         if not self._seqs:
             raise RuntimeError("activate the sequences first")
         if n_new <= 0 or max(self.lengths[s] for s in self._seqs) + n_new > self.max_seq_len:
@@ -210,7 +211,13 @@ class SharedPrefixFP8Fp8Cache:
         self._bt, self._lens = self.table.block_table[at], self.table.seq_lens[at]
         self._counts = self._lens - self._positions   # 0 where there were no pages: nothing is written then
 
+    def _not_captured(self) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a SharedPrefixFP8Fp8Cache follows its sequences on the host: a graph would replay the lengths and table "
+                               "of the step that was captured.  PageTable, append and decode can be captured")
+
     def _extended(self) -> None:
+        self._not_captured()
         if self._new == 0:
             raise RuntimeError("extend first: the active sequences or their pages changed since")
 

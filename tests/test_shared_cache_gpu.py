@@ -376,6 +376,24 @@ def test_a_refused_model_call_leaves_the_cache_as_it_was():
     other.check()
 
 
+def test_capture_is_refused(monkeypatch):
+    """A replay would use the host's lengths of the captured step."""
+    cache = SharedPrefixFP8Fp8Cache(2, 2, 256, num_layers=1)
+    kv, q = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, 4, 128, dtype=torch.bfloat16, device="cuda")
+    cache.activate([0])
+    cache.extend(1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: cache.extend(1), lambda: cache.update(kv, kv, 0), lambda: cache.decode(q, 0), cache.positions):
+        with pytest.raises(RuntimeError, match="captured"):
+            call()
+    assert cache.lengths == [1, 0]
+    monkeypatch.undo()
+    cache.update(kv, kv, 0)
+    cache.decode(q, 0)
+    assert cache.table.seq_lens.tolist() == [1, 0]
+    cache.check()
+
+
 def test_driver_with_samples():
     r = subprocess.run([sys.executable, "-m", "ffa_speedtest_b200.fp8fp8.e2e.bench_llama_fp8fp8", "--context", "300", "--samples", "3",
                         "--decode-steps", "70", "--batch", "2", "--iters", "2", "--warmup", "1", "--json"], cwd=ROOT, capture_output=True,
