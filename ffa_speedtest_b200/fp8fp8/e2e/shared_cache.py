@@ -20,7 +20,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
-from ...pages import PageTable, append_ragged_fp8fp8
+from ...pages import PageTable, append_ragged_fp8fp8, upload
 from ..attn_kernel.attn_kernel_shared_prefix_fp8fp8 import SharedPrefixWorkspace, attn_forward_decode_shared_prefix_fp8fp8
 from .fp8fp8_cache import PAGE, resolve_fp8_dtype
 
@@ -98,7 +98,7 @@ class SharedPrefixFP8Fp8Cache:
         if not seqs:
             raise ValueError("activate at least one sequence")
         self._seqs = seqs
-        self._rows = torch.tensor(seqs, dtype=torch.int32, device=self.device)
+        self._rows = upload(seqs, self.device)
         self._slice = slice(seqs[0], seqs[0] + len(seqs)) if seqs == list(range(seqs[0], seqs[0] + len(seqs))) else None
         self._new = 0
         self._group()
@@ -120,8 +120,8 @@ class SharedPrefixFP8Fp8Cache:
         rows = self._contents[self._seqs, :cols]
         same = (rows[1:] == rows[:-1]) & (np.arange(cols) < np.minimum(lens[1:], lens[:-1])[:, None])
         start, pages = _stretches(np.where(same.all(1), cols, same.argmin(1)))      # the first page that is not the next one's too
-        self._group_start = torch.tensor(start, dtype=torch.int32, device=self.device)
-        self._prefix_pages = torch.tensor(pages, dtype=torch.int32, device=self.device)
+        self._group_start = upload(start, self.device)
+        self._prefix_pages = upload(pages, self.device)
 
     def fork(self, parents: Sequence[int], children: Sequence[int]) -> None:
         """Let the empty sequences ``children[i]`` begin with the tokens of ``parents[i]``, on the same pages."""

@@ -24,12 +24,21 @@ BAD_ARGUMENT, NO_SPACE = 1, 2           # bits of PageTable.status()
 Numbers = Union[torch.Tensor, Sequence[int]]
 
 
+def upload(numbers: Sequence[int], device: torch.device) -> torch.Tensor:
+    """An int32 vector on the device, without waiting for what the stream still has to do: through pinned memory, which
+    the allocator keeps until the copy is over."""
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("a graph would keep the numbers of a list: give a device tensor while a stream is captured")
+    return torch.tensor(list(numbers), dtype=torch.int32).pin_memory().to(device, non_blocking=True)
+
+
 class PageTable:
     """Block table ``[max_seqs, pages_per_seq]``, lengths and reference counts of the pages of ``pools``.
 
     ``pools``: the tensors ``[n_pages, 64, ...]`` whose page ``p`` belongs to cache page ``p`` (base, residual and V
     of every layer that shares the table); ``extend`` and ``compact`` copy pages in all of them.  Lists of sequence
-    numbers and lengths are int32 device tensors or Python sequences (which are copied to the device first).
+    numbers and lengths are int32 device tensors or Python sequences (which are copied to the device first, without
+    waiting for it).
 
     A call that cannot be carried out changes nothing and sets a bit of the status word: ``BAD_ARGUMENT`` or
     ``NO_SPACE``.  ``check()`` raises for it.  Calls on one table must not overlap on the GPU: keep them on one
@@ -97,7 +106,7 @@ class PageTable:
 
     def _list(self, x: Numbers, name: str) -> torch.Tensor:
         if not isinstance(x, torch.Tensor):
-            x = torch.tensor(list(x), dtype=torch.int32, device=self.device)
+            x = upload(x, self.device)
         if x.dtype != torch.int32 or x.dim() != 1 or x.device != self.device or not x.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 vector on {self.device}")
         if x.numel() > self.max_seqs:

@@ -195,6 +195,27 @@ def test_compact_beside_the_state():
         t.compact(block_table_out=out[:, :5], refcount_out=count)
 
 
+def test_empty_lists_do_nothing():
+    t, m = make(10, 4, 4)
+    both(t, m, "extend", [0], [70])
+    for what, *args in (("extend", [], []), ("truncate", [], []), ("fork", [], [])):
+        both(t, m, what, *args)
+    t.free([])
+    t.extend([], 3)
+    m.same_as(t)
+
+
+def test_lists_are_refused_while_a_graph_is_captured(monkeypatch):
+    t, m = make(10, 4, 4)
+    both(t, m, "extend", [0], [70])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: t.extend([0], 1), lambda: t.truncate([0], [1]), lambda: t.fork([0], [1]), lambda: t.free([0])):
+        with pytest.raises(ValueError, match="device tensor"):
+            call()
+    monkeypatch.undo()
+    m.same_as(t)
+
+
 def test_wrapped_slice_and_other_stream():
     from ffa_speedtest_b200.pages import PageTable
     big = torch.full((7, 20), 99, dtype=torch.int32, device="cuda")

@@ -376,6 +376,33 @@ def test_a_refused_model_call_leaves_the_cache_as_it_was():
     other.check()
 
 
+def test_nothing_waits_for_the_device():
+    """Sequences come and go and steps are taken without a copy or a question that waits for the stream."""
+    cache = SharedPrefixFP8Fp8Cache(6, 2, 256, num_layers=1)
+    kv, q = torch.zeros(3, 1, 2, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(3, 1, 4, 128, dtype=torch.bfloat16, device="cuda")
+    prompt = torch.zeros(1, 100, 2, 128, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        cache.activate([0])
+        cache.extend(100)
+        cache.update(prompt, prompt, 0)
+        cache.fork([0, 0, 0], [1, 2, 4])
+        for seqs in ([1, 2, 4], [0, 1, 2]):                 # side by side in the table, and not
+            cache.activate(seqs)
+            cache.extend(1)
+            cache.positions()
+            cache.update(kv, kv, 0)
+            cache.decode(q, 0)
+        cache.truncate([1, 2], [90, 70])
+        cache.free([4])
+        cache.compact()
+        cache.table.extend([0], 1)
+        cache.table.truncate([0], [5])
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    cache.check()
+
+
 def test_capture_is_refused(monkeypatch):
     """A replay would use the host's lengths of the captured step."""
     cache = SharedPrefixFP8Fp8Cache(2, 2, 256, num_layers=1)
