@@ -77,9 +77,11 @@ class SharedPrefixFP8Fp8Cache:
         self.device = self.table.device
         self.lengths = [0] * max_seqs
         # what is in every page of every sequence: equal numbers in a column are one page, a page gets a new number when
-        # it is written to
+        # it is written to.  Known up to so many tokens of a sequence, what was written since is its own (`_note`)
         self._contents = np.full((max_seqs, pages_per_seq), -1, dtype=np.int64)
+        self._known = [0] * max_seqs
         self._next_content = 0
+        self._groups: Optional[tuple[torch.Tensor, torch.Tensor]] = None
         self._seqs: list[int] = []
         self._new = 0
         self._workspace: Optional[SharedPrefixWorkspace] = None
@@ -100,28 +102,50 @@ class SharedPrefixFP8Fp8Cache:
         self._seqs = seqs
         self._rows = upload(seqs, self.device)
         self._slice = slice(seqs[0], seqs[0] + len(seqs)) if seqs == list(range(seqs[0], seqs[0] + len(seqs))) else None
-        self._new = 0
-        self._group()
+        self._new, self._groups = 0, None
 
     @property
     def active(self) -> tuple[int, ...]:
         """The sequences that ``activate`` named."""
         return tuple(self._seqs)
 
-    def _written(self, s: int, first: int, end: int) -> None:
-        """Columns first .. end - 1 of the sequence get contents of their own."""
-        self._contents[s, first:end] = np.arange(self._next_content, self._next_content + max(0, end - first))
-        self._next_content += max(0, end - first)
+    def _written(self, seqs: list[int], first: np.ndarray, end: np.ndarray) -> None:
+        """Columns first[i] .. end[i] - 1 of seqs[i] get contents of their own."""
+        n = end - first
+        at = np.arange(n.sum())
+        self._contents[np.repeat(seqs, n), at - np.repeat(n.cumsum() - n - first, n)] = self._next_content + at
+        self._next_content += len(at)
 
-    def _group(self) -> None:
-        """Stretches of the batch whose sequences have their first full pages in common, and how many."""
-        lens = np.array([self.lengths[s] for s in self._seqs], dtype=np.int64) // PAGE
-        cols = max(1, int(lens.max()))
-        rows = self._contents[self._seqs, :cols]
-        same = (rows[1:] == rows[:-1]) & (np.arange(cols) < np.minimum(lens[1:], lens[:-1])[:, None])
-        start, pages = _stretches(np.where(same.all(1), cols, same.argmin(1)))      # the first page that is not the next one's too
-        self._group_start = upload(start, self.device)
-        self._prefix_pages = upload(pages, self.device)
+    def _note(self, seqs: Sequence[int]) -> None:
+        """Give a number to what the sequences wrote since it was last asked for."""
+        grown = [s for s in seqs if self.lengths[s] > self._known[s]]
+        if grown:
+            of = lambda x: np.array([x[s] for s in grown], dtype=np.int64)
+            self._written(grown, of(self._known) // PAGE, -(-of(self.lengths) // PAGE))
+            for s in grown:
+                self._known[s] = self.lengths[s]
+
+    def _group(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """Stretches of the batch whose sequences have their first full pages in common, and how many: asked for by the next
+        step, so that several changes in a row cost it once."""
+        if self._groups is None:
+            self._note(self._seqs)
+            lens = np.array([self.lengths[s] for s in self._seqs], dtype=np.int64) // PAGE
+            cols = max(1, int(lens.max()))
+            rows = self._contents[self._seqs, :cols]
+            same = (rows[1:] == rows[:-1]) & (np.arange(cols) < np.minimum(lens[1:], lens[:-1])[:, None])
+            start, pages = _stretches(np.where(same.all(1), cols, same.argmin(1)))  # the first page that is not the next one's too
+            both = upload([*start, *pages], self.device)
+            self._groups = both[:len(start)], both[len(start):]
+        return self._groups
+
+    @property
+    def _group_start(self) -> torch.Tensor:
+        return self._group()[0]
+
+    @property
+    def _prefix_pages(self) -> torch.Tensor:
+        return self._group()[1]
 
     def fork(self, parents: Sequence[int], children: Sequence[int]) -> None:
         """Let the empty sequences ``children[i]`` begin with the tokens of ``parents[i]``, on the same pages."""
@@ -131,10 +155,12 @@ class SharedPrefixFP8Fp8Cache:
         if any(self.lengths[c] for c in children):
             raise ValueError("the children must be empty: free them first")
         self.table.fork(parents, children)
+        self._note(dict.fromkeys(parents))
         for p, c in zip(parents, children):
-            self.lengths[c], self._contents[c] = self.lengths[p], self._contents[p]
-        if self._seqs:
-            self._group()
+            held = -(-self.lengths[p] // PAGE)
+            self._contents[c, :held] = self._contents[p, :held]
+            self.lengths[c] = self._known[c] = self.lengths[p]
+        self._groups = None
 
     def truncate(self, seqs: Sequence[int], new_lens: Sequence[int]) -> None:
         """Drop the tokens past ``new_lens`` (rejected drafts)."""
@@ -142,18 +168,20 @@ class SharedPrefixFP8Fp8Cache:
         if len(new_lens) != len(seqs) or any(n < 0 for n in new_lens):
             raise ValueError("truncate takes one length for each sequence")
         self.table.truncate(seqs, new_lens)
+        alone = []
         for s, n in zip(seqs, new_lens):
-            if n < self.lengths[s]:
-                full, held = n // PAGE, -(-n // PAGE)
+            if n < self._known[s]:
                 # cut back into pages that others hold too it goes on by itself: kept with them, it would hold down what
                 # all of them read once
-                if full < self.lengths[s] // PAGE and np.count_nonzero(self._contents[:, full] == self._contents[s, full]) > 1:
-                    self._written(s, 0, held)
-                self._contents[s, held:] = -1
-                self.lengths[s] = n
-        self._new = 0
-        if self._seqs:
-            self._group()
+                full = n // PAGE
+                if 0 < n and full < self._known[s] // PAGE and np.count_nonzero(
+                        (self._contents[:, full] == self._contents[s, full]) & (np.array(self._known) // PAGE > full)) > 1:
+                    alone.append(s)
+                self._known[s] = n
+            self.lengths[s] = min(self.lengths[s], n)
+        if alone:
+            self._written(alone, np.zeros(len(alone), dtype=np.int64), np.array([-(-self.lengths[s] // PAGE) for s in alone]))
+        self._new, self._groups = 0, None
 
     def free(self, seqs: Sequence[int]) -> None:
         """End the sequences and give their pages back."""
@@ -178,9 +206,7 @@ class SharedPrefixFP8Fp8Cache:
             held = np.arange(rows.shape[1]) < -(-np.array(self.lengths)[:, None] // PAGE)
             self._contents = np.where(held & (rows >= 0), rows + self._next_content, -1)
             self._next_content += self.table.n_pages
-            self._new = 0
-            if self._seqs:
-                self._group()
+            self._known, self._new, self._groups = list(self.lengths), 0, None
             raise
         if self._workspace is not None:
             self._gave_up |= self._workspace.status_word
@@ -206,7 +232,6 @@ class SharedPrefixFP8Fp8Cache:
         self.table.extend(self._rows, n_new)
         self._new = n_new
         for s in self._seqs:
-            self._written(s, self.lengths[s] // PAGE, -(-(self.lengths[s] + n_new) // PAGE))
             self.lengths[s] += n_new
         self._bt, self._lens = self.table.block_table[at], self.table.seq_lens[at]
         self._counts = self._lens - self._positions   # 0 where there were no pages: nothing is written then

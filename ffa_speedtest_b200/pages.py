@@ -114,6 +114,10 @@ class PageTable:
         return x
 
     def _pair(self, seqs: Numbers, name: str, values, value_name: str):
+        if not isinstance(seqs, torch.Tensor) and not isinstance(values, (torch.Tensor, int)):
+            seqs, values = list(seqs), list(values)
+            both = upload([*seqs, *values], self.device)      # one copy for two lists
+            seqs, values = both[:len(seqs)], both[len(seqs):]
         seqs = self._list(seqs, name)
         if isinstance(values, int):
             values = torch.full_like(seqs, values)
