@@ -118,16 +118,16 @@ __global__ void __launch_bounds__(1024) sp_merge_kernel(const __grid_constant__ 
   if (me.group_tiles > 0) {
     const int all = (b - me.group_first) * p.G + g, block = all / kSpRows, row = all % kSpRows;
     const int rows = min(kSpRows, me.group_rows - block * kSpRows);
-    const int x = me.group_at + (block * p.HKV + head) * sp_unit_cost(me.group_tiles) + kSpBegin;
+    const int tile = sp_tile_cost(me.group_rows), x = me.group_at + (block * p.HKV + head) * sp_unit_cost(me.group_tiles, tile) + kSpBegin;
     const int c = sp_owner(x, W, n_used);
-    n[0] = sp_owner(x + (me.group_tiles - 1) * kSpTileCost, W, n_used) - c + 1;
+    n[0] = sp_owner(x + (me.group_tiles - 1) * tile, W, n_used) - c + 1;
     const int64_t first = sp_part_row(p, false, me.group_first * p.G + block * kSpRows, rows, head, c);
     at[0] = first + row;
     o_at[0] = 32 * first + c4 * rows + row;
   }
   if (me.tiles > 0) {
-    const int x = me.at + head * sp_unit_cost(me.tiles) + kSpBegin, c = sp_owner(x, W, n_used);
-    n[1] = sp_owner(x + (me.tiles - 1) * kSpTileCost, W, n_used) - c + 1;
+    const int tile = sp_tile_cost(p.G), x = me.at + head * sp_unit_cost(me.tiles, tile) + kSpBegin, c = sp_owner(x, W, n_used);
+    n[1] = sp_owner(x + (me.tiles - 1) * tile, W, n_used) - c + 1;
     const int64_t first = sp_part_row(p, true, b * p.G, p.G, head, c);
     at[1] = first + g;
     o_at[1] = 32 * first + c4 * p.G + g;

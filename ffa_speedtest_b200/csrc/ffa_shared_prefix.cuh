@@ -19,9 +19,14 @@ constexpr int kSpTile = 128;                  // tokens of a tile: two pages
 constexpr int kSpRows = 128;                  // query rows of a unit, at most
 constexpr int kSpMaxCtas = 148;
 
-// Costs, in quarters of a tile: beginning a unit (q, the first loads' latency, its partials), and a tile.  Over 28 batches
-// of mixed shapes 4, 5, 6 and 8 for the first gave 34.6, 34.3, 34.1 and 34.4 us in geometric mean.
-constexpr int kSpBegin = 6, kSpTileCost = 4;
+// Costs, in quarters of a tile of few rows: beginning a unit (q, the first loads' latency, its partials), a tile of up to 64
+// query rows, a tile of more (the exponentials of 128 rows, and with bfloat16 V twice the MMAs of P V; 1.9 us where a tile of
+// few rows takes 1.4).  Over 28 batches of mixed shapes 4, 5, 6 and 8 for the first gave 34.6, 34.3, 34.1 and 34.4 us in
+// geometric mean.  4, 5, 6 and 7 for the last: 64 samples of 128K 294, 267, 286 and 307 us, 32 samples of 16K in fp16 45.9,
+// 44.0, 43.4 and 46.4, the 28 batches the same within 0.7 %.
+constexpr int kSpBegin = 6, kSpNarrowTile = 4, kSpWideTile = 5;
+// a tile of an item with so many query rows to a kv-head
+__host__ __device__ inline int sp_tile_cost(int rows) { return rows > 64 ? kSpWideTile : kSpNarrowTile; }
 
 // where the merge finds the partials of a sequence's rows: the places of its item and of its group's on the line
 struct SpSequence {
@@ -77,14 +82,17 @@ __device__ __forceinline__ int64_t sp_part_row(const SpParams& p, bool own, int 
   return own ? sp_shared_rows(p.B, p.HQ) + at + static_cast<int64_t>(cta) * p.G : at + static_cast<int64_t>(cta) * kSpRows;
 }
 
-// Cost of a unit of so many tiles.  Tile t of a unit that begins at U stands at U + kSpBegin + t * kSpTileCost.
-__device__ __forceinline__ int sp_unit_cost(int tiles) { return tiles > 0 ? kSpBegin + tiles * kSpTileCost : 0; }
-// The line is at most this long (the host refuses what could give 2^31 or more).
+// Cost of a unit of so many tiles.  Tile t of a unit that begins at U stands at U + kSpBegin + t * tile_cost.
+__device__ __forceinline__ int sp_unit_cost(int tiles, int tile_cost) { return tiles > 0 ? kSpBegin + tiles * tile_cost : 0; }
+// The line is at most this long (the host refuses what could give 2^31 or more): every sequence and every group a unit of few
+// rows, and what groups of more rows cost beyond that, which is most for a row if a group has one row more than a block.
 __host__ __device__ inline int64_t sp_longest_line(int64_t B, int64_t NG, int64_t HKV, int64_t G, int64_t cols) {
-  return HKV * (kSpBegin + (cols + 1) / 2 * kSpTileCost) * (B + NG + B * G / kSpRows);
+  const int64_t tiles = (cols + 1) / 2;
+  return HKV * ((B + NG) * (kSpBegin + tiles * kSpNarrowTile) +
+                B * G * (kSpBegin + tiles * (2 * kSpWideTile - kSpNarrowTile)) / kSpRows);
 }
-// CTAs that take part on a line of length W: each gets 4 at least, a tile, so that every CTA between the first and the
-// last of a unit has a tile of it (8 on average, less what rounding takes).  CTA c begins at c * (W / n).
+// CTAs that take part on a line of length W: each gets 8 on average, 7 at least after rounding, more than a tile, so that
+// every CTA between the first and the last of a unit has a tile of it.  CTA c begins at c * (W / n).
 __device__ __forceinline__ int sp_ctas(int W, int n_ctas) { return max(1, min(n_ctas, W / 8)); }
 __device__ __forceinline__ int sp_first(int c, int W, int n) {
   return c >= n ? W : static_cast<int>(static_cast<float>(c) * (static_cast<float>(W) * __frcp_rn(static_cast<float>(n))));

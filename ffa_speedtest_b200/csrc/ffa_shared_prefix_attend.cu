@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     const int i = i0 + tid;
     SpItem x{};
     if (i < n_items) x = sp_item(p, bounds, i, i0 == 0 ? first_len : i < p.B ? p.seq_lens[i] : 0);
-    const int cost = x.units * sp_unit_cost(x.tiles);
+    const int cost = x.units * sp_unit_cost(x.tiles, sp_tile_cost(x.rows));
     int sum;
     const int at = W + cta_exclusive(cost, s_plan, sum);
     if (i0 == 0) { mine = x; my_cost = cost; my_at = at; first_sum = sum; }
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
       const int i = i0 + tid;
       SpItem x{};
       if (i < n_items) x = sp_item(p, bounds, i, i < p.B ? p.seq_lens[i] : 0);
-      const int cost = x.units * sp_unit_cost(x.tiles);
+      const int cost = x.units * sp_unit_cost(x.tiles, sp_tile_cost(x.rows));
       int sum;
       const int at = before + cta_exclusive(cost, s_plan, sum);
       before += sum;
@@ -768,15 +768,15 @@ __global__ void __launch_bounds__(kThreads, 1) sp_attend_mma_kernel(const __grid
     int place = s_plan[13];
     // the runs of one item
     auto runs_of = [&](const SpItem& it, bool own) -> bool {
-      const int unit = sp_unit_cost(it.tiles), before = x0 - place - kSpBegin - (it.tiles - 1) * kSpTileCost;
+      const int tile = sp_tile_cost(it.rows), unit = sp_unit_cost(it.tiles, tile), before = x0 - place - kSpBegin - (it.tiles - 1) * tile;
       int k = before <= 0 ? 0 : (before - 1) / unit + 1;                          // units that end before x0 are other CTAs'
       int block = k / p.HKV, head = k - block * p.HKV;
 #pragma unroll 1
       for (; k < it.units; ++k) {
         const int first = place + k * unit + kSpBegin;                            // where tile 0 stands
         if (first >= x1) break;
-        const int t0 = first >= x0 ? 0 : (x0 - first - 1) / kSpTileCost + 1;
-        const int t1 = min(it.tiles, (x1 - first - 1) / kSpTileCost + 1);
+        const int t0 = first >= x0 ? 0 : (x0 - first - 1) / tile + 1;
+        const int t1 = min(it.tiles, (x1 - first - 1) / tile + 1);
         Run r;
         r.table_row = it.first;
         r.head = head;
