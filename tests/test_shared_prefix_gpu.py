@@ -280,6 +280,16 @@ def test_large_batch():
     b.check(b.call())
 
 
+def test_largest_batch():
+    from ffa_speedtest_b200.fp8fp8.attn_kernel.attn_kernel_shared_prefix_fp8fp8 import SharedPrefixWorkspace
+    sizes = [1] * 900 + [2, 3] * 600 + [196]
+    b = Batch(sizes, [(i % 3 + 1) // 2 for i in range(len(sizes))], [0, 1, 5, 64, 70], 2, 1, seed=19)
+    assert b.B == 4096
+    b.check(b.call())
+    with pytest.raises(ValueError, match="1 to 4096"):
+        SharedPrefixWorkspace(4097, 2, 1, b.q.device, b.q.dtype)
+
+
 def test_same_as_the_pruned_decode_that_drops_nothing():
     from ffa_speedtest_b200.fp8fp8.attn_kernel.attn_kernel_v1210_fused_bsz_fp8fp8 import attn_forward_decode_fp8fp8
     b = Batch([4], [30], [100], 32, 8, seed=9)
