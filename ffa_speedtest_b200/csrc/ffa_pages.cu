@@ -8,9 +8,9 @@
 // changes nothing and sets a bit of `status`.
 //
 // Cost: the bookkeeping is a few KiB to a few hundred KiB in L2 and bound by latency; the page copies are bound by
-// HBM (every byte read once and written once).  Measured: truncate, fork and extend for 4 samples of 1K tokens 16.5 us
-// together, 4 us a launch; for 64 samples of 32K and 8 layers (open pages copied: 87 MB read, 87 MB written) 45 us, 25 of
-// them the copy; compact of 2000 pages in 4 layers 197 us for 1.04 GB, 5.3 TB/s.
+// HBM (every byte read once and written once).  Measured as graphs: truncate, fork and extend for 4 samples of 1K tokens
+// 13.7 us together, 3.4 a launch; for 64 samples of 32K and 8 layers (open pages copied: 87 MB read, 87 MB written) 44 us, 25
+// of them the copy; compact of 2000 pages in 4 layers 196 us for 1.04 GB, 5.3 TB/s.
 #include "ffa_common.cuh"
 
 namespace ffa {

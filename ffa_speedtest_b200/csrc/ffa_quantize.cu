@@ -373,8 +373,8 @@ __global__ void __launch_bounds__(256) nvfp4_kernel(const void* __restrict__ k, 
 
 // K and V of new tokens to each sequence's own position.  A block takes kAppendRows tokens of one sequence, a thread
 // eight channels of a token at a time: quantises K, copies V; the loads of four are in flight per thread.  Bound by HBM
-// (512 bytes read and 512 written per token and kv-head): 8 prompts of up to 8191 tokens, 476 MB, 86 us, 5.6 TB/s (80 us
-// at full clocks); one token for each of 64 sequences 4.2 us, a launch.  Tokens past counts[b], and positions without a page, are left
+// (512 bytes read and 512 written per token and kv-head): 8 prompts of up to 8191 tokens, 476 MB, 80 us, 5.9 TB/s (86 us
+// among other calls); one token for each of 64 sequences 4.1 us, a launch.  Tokens past counts[b], and positions without a page, are left
 // out: nothing is written for them.
 constexpr int kAppendRows = 16;
 template <int DT, int F8>

@@ -58,8 +58,9 @@ __device__ void split_q(const SpParams& p, int64_t row_id) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = finite ? x[e] * mul : 0.f;
   if (!live) return;
-  // infinities and NaN in q or in the softmax scale make the whole row NaN; the scale stays above zero, so that the -inf of a masked token times it
-  // is -inf (1e-30 times a dot product of pieces, below 2^28, is nothing in a score)
+  // infinities and NaN in q or in the softmax scale make the whole row NaN; the scale stays above zero, so that the -inf of a
+  // masked token times it is -inf (1e-30 times a dot product of pieces, 128 times 2^8 times base and residual of up to 57344
+  // and so below 2^32, is nothing in a score)
   if ((lane & 7) == 0)
     p.q_scale[row_id] = finite ? fmaxf(fabsf(p.scale_log2) * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), 1e-30f) : NAN;
   for (int piece = 0; piece < p.pieces; ++piece) {
@@ -313,7 +314,8 @@ extern "C" int ffa_decode_shared_prefix(const FfaSharedPrefixArgs* a, ffa_stream
   int rc = last_launch("ffa_decode_shared_prefix (q)");
   if (rc) return rc;
   if ((rc = launch_sp_attend(p, st))) return rc;
-  // the merge's blocks are set up while the attention still runs; they wait for its end before they read
+  // the merge is launched while the attention still runs: its blocks start on SMs whose CTA has ended (both do not fit on one)
+  // and wait there for the end of the others
   const int64_t pairs = static_cast<int64_t>(p.B) * p.HKV;
   const int slices = pairs * 4 <= p.n_ctas ? 4 : pairs * 2 <= p.n_ctas ? 2 : 1;
   const int64_t per_sm = (pairs * slices + p.n_ctas - 1) / p.n_ctas;

@@ -11,17 +11,22 @@
 // the raw base and residual bytes accumulate into one fp32 tile.  That costs 4 (6) times the fp8 MMAs of one product,
 // twice (three times) what a dequantised 16-bit K would, but K never passes through registers.
 //
-// Bound: per 128 tokens and kv-head 64 KiB arrive, 2840 clocks of an SM's share of HBM at 1.9 GHz.  The tensor core needs
-// 16 (24) + 8 MMAs of 64 clocks a step.  The softmax of a row takes 128 exponentials, 1024 clocks of the special-function
-// unit of a quarter of the SM, and some 600 clocks around them (exponentials by a polynomial on the FMA units were tried:
-// half of them so made a step 600 clocks longer).  Measured, with the kernels before and after (bf16, 8 kv-heads, 4 query
-// heads to each): 8 samples of 32K tokens 39 us for 147 MB, of which 4 until the first tile; 16 sequences that share
-// nothing 83 us for 400 MB, 4.8 TB/s; 64 samples of 128K 312 us (243 without a load before it): 256 rows are two units,
-// each of which reads the prompt, 1353 MB at 5.6 TB/s and an SM clock that the power limit holds at 1.6 GHz and below.
-// One unit of 256 rows (an S and an O for each half, two softmax groups) was tried: it halves the bytes, but leaves one S
-// buffer to a half, so that S, softmax and P V follow one another: the same time there, 1 to 7 us more elsewhere.
-// S given back as soon as it is in registers, P in columns of its own (then there is room for one O only): 3 us more in
-// the smaller cases, nothing gained in the largest.
+// Bound: per 128 tokens and kv-head 64 KiB arrive, 1.48 us of an SM's share of HBM.  The tensor core needs 16 (24) + 8 MMAs
+// of 64 clocks a step, and 8 more with bfloat16 V and more than 64 rows.  The softmax of a row takes 128 exponentials, 1024
+// clocks of the special-function unit of a quarter of the SM, and some 600 clocks around them (exponentials by a polynomial
+// on the FMA units were tried: half of them so made a step 600 clocks longer).  Measured, with the kernels before and after
+// (bf16, 8 kv-heads, 4 query heads to each; in brackets a GPU under sustained load): 8 samples of 32K tokens 38.9 us (39.0)
+// for 147 MB: the first K is there after 6.4, then 1.39 a tile of 128 tokens, 3 to write O, 5 for the merge; 16 sequences that
+// share nothing 75.9 us (83.2) for 400 MB, 1.45 a tile; 64 samples of 128K 273 us (323): 256 rows are two units, each of which
+// walks the prompt, 1.8 a tile, the tensor core busy for 68 % and the power limit at 1.54 GHz; the second walk finds the
+// prompt in L2, 839 MB come from HBM.
+// One unit of 256 rows (an S and an O for each half, two softmax groups) was tried: it leaves one S buffer to a half, so
+// that S, softmax and P V follow one another: the same time there, 1 to 7 us more elsewhere.  S given back as soon as it is
+// in registers, P in columns of its own (then there is room for one O only): 3 us more in the smaller cases, nothing gained
+// in the largest.
+//
+// Code: what is executed is fetched cold at every call, and 127 KB of it took 1 to 6 us longer than 86 do, so what runs once
+// or rarely is compiled once (the walk over a unit, the long part of a wait) and its loops are not unrolled.
 //
 // Warps: 0 lists the runs and loads q, K and V; 1 issues the MMAs of S, 2 those of O (two warps, so that the waits of one
 // do not keep the other's from the tensor core); 4-7 softmax (TMEM lanes 32 * (warp % 4)).
@@ -32,7 +37,8 @@
 // (64) rows are spread over the four quarters of the TMEM lanes, eight (sixteen) to each, so that all four softmax warps
 // have work, and there four lanes share a row (softmax_16): 32 (64) exponentials a lane and not 128.  Up to 64 rows the
 // MMAs have M = 64, which takes as long as 128 but less power, and the clock rises.  16 sequences that share nothing, under
-// sustained load: 94.3 us with a row to a lane and M = 128, 92.5 spread, 83.3 with M = 64.
+// sustained load, with one bfloat16 to a weight: 94.3 us with a row to a lane and M = 128, 92.5 spread, 83.3 with M = 64.
+// The second pieces of bfloat16 weights have the lanes eight (sixteen) further on; with 33 to 64 rows their MMA has M = 128.
 //
 // The line of costs does not depend on the kernel that splits q, nor do K and V: both are begun while that one runs.
 //
@@ -276,9 +282,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {       // NaN 
 }
 // Weights as the MMA takes them, two tokens to a word.  float16: eleven bits.  bfloat16 has only eight, so there a weight is
 // two of them, the leading eight bits (cut off) and the rest, rounded to eight more: sixteen bits.  Up to 64 query rows the
-// rest has rows of the MMA to itself that were idle; with more the MMAs of P V are issued twice.  One piece would be faster,
-// by 38.3 to 39.0 us (8 samples of 32K), 40.1 to 41.6 (ragged prompts), 74.3 to 75.8 (16 private) and, with 128 rows, 260 to
-// 296 (64 samples of 128K); but its rounding is as large as that of a bfloat16 output, and larger than that of any other.
+// rest has rows of the MMA to itself that were idle; with more the MMAs of P V are issued twice.  One piece is faster,
+// 38.3 to 39.0 us (8 samples of 32K), 40.1 to 41.6 (ragged prompts), 74.3 to 75.8 (16 private) and, with 128 rows, 260 to 296
+// (64 samples of 128K, all tiles counted alike); but its rounding is as large as that of a bfloat16 output, and larger than
+// that of any other.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float2 w) {
   uint32_t r;

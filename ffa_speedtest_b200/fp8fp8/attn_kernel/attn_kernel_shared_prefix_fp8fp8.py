@@ -18,7 +18,8 @@ _SCALE = 1.0 / math.sqrt(128)
 
 class SharedPrefixWorkspace:
     """Output and scratch of the shared-prefix decode, for one batch size and head layout.  One call at a time may
-    use it (two captured graphs that may run at the same time need one each)."""
+    use it (two captured graphs that may run at the same time need one each).  It is zeroed on the stream that is current
+    when it is made: calls on another stream have to come after that."""
 
     def __init__(self, B: int, HQ: int, HKV: int, device, dtype):
         self.B, self.HQ, self.HKV, self.device, self.dtype = int(B), int(HQ), int(HKV), torch.device(device), dtype
@@ -66,7 +67,8 @@ def attn_forward_decode_shared_prefix_fp8fp8(
     from the table row of the group's first sequence.  ``seq_lens`` counts all tokens of a sequence, shared ones
     included; a sequence of length 0 gives zeros, one that is shorter than its group's prefix sees its own tokens only (V
     of the others has to be finite there).  Lengths and groups are read on the device when the kernels run.
-    ``partial_out [B, HQ, 129]`` (fp32) also receives the normalised output and the base-2 log-sum-exp."""
+    ``partial_out [B, HQ, 129]`` (fp32) also receives the normalised output and the base-2 log-sum-exp.  Without ``out`` the
+    result is the workspace's own buffer, which its next call overwrites."""
     if not (q.is_cuda and k_fp8.is_cuda and v.is_cuda):
         raise ValueError("q, K and V must be CUDA tensors (this build has no CPU path)")
     q_shape, k_shape = q.shape, k_fp8.shape

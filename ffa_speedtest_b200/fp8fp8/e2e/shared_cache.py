@@ -8,8 +8,9 @@ pages once per group of sequences (every token counts; nothing is pruned).
 
 Sequences have numbers ``0 .. max_seqs - 1``.  ``activate`` names those that the next model calls are about, in batch
 order; sequences that were forked from one another should be next to each other in it, since a group is a stretch of
-the batch.  Lengths are known on the host as well, so that nothing here waits for the device.  A model call that runs out of
-pages writes no token; ``check()`` finds it and takes the lengths from the device again.
+the batch.  Lengths are known on the host as well, so that only ``check()`` waits for the device; for that reason model calls
+cannot be captured in a graph.  A model call that runs out of pages writes no token; ``check()`` finds it and takes lengths
+and shared pages from the device again.
 
 The reference has no counterpart (ffa-fp8fp8/e2e/fp8fp8_cache.py appends a batch of one length with ``torch.cat``).
 """
@@ -260,7 +261,8 @@ class SharedPrefixFP8Fp8Cache:
                              self.key_residual[layer_idx], self.value[layer_idx], self._bt, self._positions, self._counts)
 
     def decode(self, q: torch.Tensor, layer_idx: int, scale: Optional[float] = None) -> torch.Tensor:
-        """Attention of ``q [B, 1, HQ, 128]`` over all tokens of its sequence -> ``[B, HQ, 128]``."""
+        """Attention of ``q [B, 1, HQ, 128]`` over all tokens of its sequence -> ``[B, HQ, 128]``, a buffer that the next
+        call overwrites."""
         self._extended()
         ws = self._workspace
         if ws is None or not ws.matches(q.shape[0], q.shape[2], self.num_kv_heads, q.device, q.dtype):

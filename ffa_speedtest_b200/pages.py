@@ -41,8 +41,8 @@ class PageTable:
     waiting for it).
 
     A call that cannot be carried out changes nothing and sets a bit of the status word: ``BAD_ARGUMENT`` or
-    ``NO_SPACE``.  ``check()`` raises for it.  Calls on one table must not overlap on the GPU: keep them on one
-    stream, or order the streams."""
+    ``NO_SPACE``.  ``check()`` raises for it.  Calls on one table must not overlap on the GPU, nor with the table's
+    own making (which zeroes its scratch): keep them on one stream, or order the streams."""
 
     def __init__(self, n_pages: int, max_seqs: int, pages_per_seq: int, *, pools: Sequence[torch.Tensor] = (),
                  device="cuda"):

@@ -297,7 +297,7 @@ typedef struct FfaPagePools {
   const int32_t* token_bytes;
 } FfaPagePools;
 size_t ffa_pages_scratch_bytes(int32_t n_pages, int32_t max_seqs);
-/* Shortens sequences seqs[i] to new_lens[i] tokens (0 ends one); a length above the present one changes nothing.
+/* Shortens sequences seqs[i] to new_lens[i] >= 0 tokens (0 ends one); one above the present length changes nothing.
  * Pages past the new length lose this holder.  A sequence may be listed twice: the smaller length holds. */
 int ffa_pages_truncate(const FfaPageTable* table, const int32_t* seqs, const int32_t* new_lens, int32_t n,
                        ffa_stream_t stream);
@@ -327,7 +327,9 @@ int ffa_pages_compact(const FfaPageTable* table, const FfaPagePools* pools, int3
  * sequence outside every group has no shared part, nor has any if the bounds do not ascend.  All of this is device
  * memory and is read by the kernels, so a captured call follows it.  Entries outside 0 .. n_pages - 1 read as zero keys
  * and values.  V that a sequence of a group does not see but another one does (a sequence shorter than the prefix) has
- * to be finite.  A row of q that is not finite, or an sm_scale that is not, gives NaN.  At most 4096 sequences; a batch
+ * to be finite.  A row of q that is not finite, or an sm_scale that is not, gives NaN, unless its sequence has
+ * length 0.  Scores (q . k * sm_scale) have to be below 2^26 in magnitude: beyond, fp32 does not resolve the difference
+ * of two of them.  Weights are held in 11 bits where V is float16 and in 16 where it is bfloat16, sums in fp32.  At most 4096 sequences; a batch
  * whose table could hold more work than 2^31 units (4 per 128 tokens, kv-head and block of 128 query rows) gives
  * FFA_E_LIMIT.  The reference has no counterpart (its sequences share nothing).
  */
