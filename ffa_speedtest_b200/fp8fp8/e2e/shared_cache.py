@@ -65,8 +65,14 @@ class SharedPrefixFP8Fp8Cache:
             raise ValueError(f"this build supports head_dim 128, got {head_dim}")
         if num_layers <= 0:
             raise ValueError(f"num_layers must be positive, got {num_layers}")
+        if num_kv_heads <= 0:
+            raise ValueError(f"num_kv_heads must be positive, got {num_kv_heads}")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be float16 or bfloat16, got {dtype}")
         self.num_kv_heads, self.head_dim, self.num_layers, self.dtype = num_kv_heads, head_dim, num_layers, dtype
         self.fp8_dtype = fp8_dtype or resolve_fp8_dtype(device)
+        if self.fp8_dtype not in (torch.float8_e4m3fn, torch.float8_e5m2):
+            raise ValueError(f"fp8_dtype must be float8_e4m3fn or float8_e5m2, got {self.fp8_dtype}")
         pages_per_seq = -(-max_seq_len // PAGE)
         self.max_seq_len = pages_per_seq * PAGE
         shape = (n_pages or max_seqs * pages_per_seq, PAGE, num_kv_heads, head_dim)
